@@ -26,6 +26,8 @@ __all__ = [
     "matmul_bf16_gpu_batched_deferred", "flush", "DeviceBuffer", "gemv_cs", "gemv_rd",
     "synchronize", "probe_read", "gemv_rd_grouped", "fill_counter_bf16", "Graph", "Event", "plan", "register_weight", "release_weights",
     "resident_count", "resident_bytes", "device_info", "vault_load_npz", "npz_locate", "f16_upconvert",
+    "mxfp4_row", "mxfp4_quantize", "mxfp4_dequantize", "gemv_mxfp4_rd", "gemm_mxfp4",
+    "KV8Cache", "KV8Batch", "kv8_append", "kv8_attend",
 ]
 
 MIN_MACS = 1 << 14  # DMC_HIP_MIN_MACS in include/dmc_hip.h
@@ -279,6 +281,95 @@ def f16_upconvert(src, dst, n: int) -> None:
     """Enqueue dst f32[n] = the IEEE f16 patterns src[n] widened exactly
     (f16_bits_to_f32, jit.rs:29231-29257)."""
     _lib.check(_lib.load().dmc_hip_f16_upconvert(_addr(src), _addr(dst), n))
+
+
+# ---- 4-bit weights (MXFP4) and the 8-bit attention cache --------------------------------
+
+DTYPES = {"f32": 0, "bf16": 1}  # DMC_HIP_F32, DMC_HIP_BF16
+
+
+def _dtype(name: str) -> int:
+    if name not in DTYPES:
+        raise ValueError(f"dtype must be one of {sorted(DTYPES)}, got {name!r}")
+    return DTYPES[name]
+
+
+def mxfp4_row(k: int) -> tuple[int, int]:
+    """(code bytes, scale bytes) of a row of k values in MXFP4."""
+    lib = _lib.load()
+    return int(lib.dmc_hip_mxfp4_row_bytes(k)), int(lib.dmc_hip_mxfp4_row_scales(k))
+
+
+def mxfp4_quantize(src, q, scales, rows: int, k: int, dtype: str = "f32", ld: int = 0) -> None:
+    """Enqueue rows [rows, k] (ld elements apart, 0: k) to MXFP4 codes and scales, rows mxfp4_row(k) bytes apart."""
+    _lib.check(_lib.load().dmc_hip_mxfp4_quantize(_addr(src), _dtype(dtype), ld, _addr(q), _addr(scales), rows, k))
+
+
+def mxfp4_dequantize(q, scales, dst, rows: int, k: int, dtype: str = "f32", ld: int = 0) -> None:
+    """Enqueue the values that MXFP4 rows stand for into dst [rows, k]."""
+    _lib.check(_lib.load().dmc_hip_mxfp4_dequantize(_addr(q), _addr(scales), _addr(dst), _dtype(dtype), ld, rows, k))
+
+
+def gemv_mxfp4_rd(x, q, scales, y, m: int, k: int, n: int) -> None:
+    """Enqueue y = x @ W' on device regions: x f32 [m, k], W [n, k] in MXFP4, y f32 [m, n]."""
+    _lib.check(_lib.load().dmc_hip_gemv_mxfp4_rd(_addr(x), _addr(q), _addr(scales), _addr(y), m, k, n))
+
+
+def gemm_mxfp4(xq, x_scales, wq, w_scales, y, m: int, k: int, n: int) -> None:
+    """Enqueue y = X @ W' on device regions, both sides in MXFP4, y f32 [m, n]."""
+    _lib.check(_lib.load().dmc_hip_gemm_mxfp4(_addr(xq), _addr(x_scales), _addr(wq), _addr(w_scales), _addr(y),
+                                              m, k, n))
+
+
+@dataclass
+class KV8Cache:
+    """A pool of cache pages on device regions: k [pages][heads][page][dim] and v [pages][heads][dim][page] in
+    e4m3, k_scales and v_scales [pages][heads] bytes (dmc_hip_kv8)."""
+    k: object
+    v: object
+    k_scales: object
+    v_scales: object
+    pages: int
+    heads: int
+    page: int
+    dim: int
+
+    def _args(self) -> _lib.KV8:
+        return _lib.KV8(_addr(self.k), _addr(self.v), _addr(self.k_scales), _addr(self.v_scales), self.pages,
+                        self.heads, self.page, self.dim)
+
+
+@dataclass
+class KV8Batch:
+    """The sequences of a call, int32 arrays on the device: table [batch][width] page ids, lens [batch] tokens with
+    the new ones, starts [batch + 1] first row of each sequence's new tokens; max_new and max_len bound them
+    (dmc_hip_kv8_batch)."""
+    table: object
+    width: int
+    lens: object
+    starts: object
+    batch: int
+    max_new: int
+    max_len: int
+
+    def _args(self) -> _lib.KV8BatchArgs:
+        return _lib.KV8BatchArgs(_addr(self.table), self.width, _addr(self.lens), _addr(self.starts), self.batch,
+                                 self.max_new, self.max_len)
+
+
+def kv8_append(cache: KV8Cache, batch: KV8Batch, k, v, dtype: str = "f32", k_ld: int = 0, v_ld: int = 0) -> None:
+    """Enqueue the new tokens' k and v rows ([heads][dim], ld elements apart, 0: packed) into their pages."""
+    _lib.check(_lib.load().dmc_hip_kv8_append(cache._args(), batch._args(), _addr(k), _addr(v), _dtype(dtype),
+                                              k_ld, v_ld))
+
+
+def kv8_attend(cache: KV8Cache, batch: KV8Batch, q, out, q_heads: int, dtype: str = "f32",
+               scale: float | None = None, window: int = 0, q_ld: int = 0, out_ld: int = 0) -> None:
+    """Enqueue causal attention of the new tokens' q rows over the cache; scale None: dim ** -0.5, window 0: no
+    window."""
+    s = max(cache.dim, 1) ** -0.5 if scale is None else scale
+    _lib.check(_lib.load().dmc_hip_kv8_attend(cache._args(), batch._args(), _addr(q), _addr(out), _dtype(dtype),
+                                              q_heads, q_ld, out_ld, s, window))
 
 
 # ---- weight ingress ---------------------------------------------------------------

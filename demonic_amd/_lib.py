@@ -15,6 +15,18 @@ LIB_PATH = pathlib.Path(__file__).resolve().parent / "lib" / "libdmc_hip.so"
 i32, i64, f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 cstr = ctypes.c_char_p
 
+
+
+class KV8(ctypes.Structure):
+    """dmc_hip_kv8: the pool of cache pages."""
+    _fields_ = [(n, i64) for n in ("k_dev", "v_dev", "k_scales_dev", "v_scales_dev", "pages", "heads", "page", "dim")]
+
+
+class KV8BatchArgs(ctypes.Structure):
+    """dmc_hip_kv8_batch: the sequences of a call."""
+    _fields_ = [(n, i64) for n in ("table_dev", "width", "lens_dev", "starts_dev", "batch", "max_new", "max_len")]
+
+
 # name -> (restype, argtypes); one line per declaration in include/dmc_hip.h
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dmc_matmul_bf16_gpu": (None, [i64] * 6),
@@ -58,6 +70,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dmc_hip_f16_upconvert": (i32, [i64, i64, i64]),
     "dmc_hip_vault_load_npz": (i64, [cstr, cstr, i64, i64, i64]),
     "dmc_hip_npz_locate": (i32, [cstr, cstr, ctypes.POINTER(i64)]),
+    "dmc_hip_mxfp4_row_bytes": (i64, [i64]),
+    "dmc_hip_mxfp4_row_scales": (i64, [i64]),
+    "dmc_hip_mxfp4_quantize": (i32, [i64] * 7),
+    "dmc_hip_mxfp4_dequantize": (i32, [i64] * 7),
+    "dmc_hip_gemv_mxfp4_rd": (i32, [i64] * 7),
+    "dmc_hip_gemm_mxfp4": (i32, [i64] * 8),
+    "dmc_hip_kv8_append": (i32, [ctypes.POINTER(KV8), ctypes.POINTER(KV8BatchArgs)] + [i64] * 5),
+    "dmc_hip_kv8_attend": (i32, [ctypes.POINTER(KV8), ctypes.POINTER(KV8BatchArgs)] + [i64] * 6 + [f32, i64]),
     "dmc_hip_plan": (i32, [i32, i64, i64, i64, i64, i64, i64, i64, ctypes.POINTER(i64)]),
     "dmc_hip_capture_begin": (i32, []),
     "dmc_hip_capture_end": (i64, []),

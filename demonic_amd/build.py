@@ -55,6 +55,7 @@ def build_lib() -> pathlib.Path:
     cc = hipcc()
     objs = []
     for src, device in (("gemv_kernels.hip", True), ("gemm_kernels.hip", True),
+                        ("mxfp4_kernels.hip", True), ("kv8_kernels.hip", True),
                         ("dmc_hip_runtime.cpp", False), ("npz_ingress.cpp", False)):
         obj = OBJ / (src.rsplit(".", 1)[0] + ".o")
         lang = ["-x", "hip"] + DEVICE if device else ["-D__HIP_PLATFORM_AMD__"]

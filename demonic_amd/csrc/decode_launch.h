@@ -1,0 +1,94 @@
+// decode_launch.h -- host-side launch interface of the MXFP4 kernels (4-bit
+// weights and activations) and of the 8-bit attention cache's kernels.
+//
+// MXFP4: a row of k values is ceil(k / 128) groups of 128; a group is 64 bytes
+// of e2m1 codes (two to a byte, the low half first) and 4 E8M0 bytes, one per
+// block of 32.  Block b stands for code * 2^(scale - 127); byte 255 makes the
+// block NaN.  What lies past k in the last group is code 0.
+//
+// KV8: a page holds `page` tokens of every head: K as [heads][page][dim], V as
+// [heads][dim][page] (a dim's tokens lie together, as the product P V reads
+// them), e4m3 codes, with one E8M0 byte per page, head and side.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace dmc {
+
+constexpr int64_t kMxGroup = 128;  // elements of a row's group
+inline int64_t mx_groups(int64_t k) { return (k + kMxGroup - 1) / kMxGroup; }
+
+struct MxCast {
+    const void *src;  // quantise: rows at ld elements; dequantise: the codes
+    void *dst;
+    uint8_t *q;       // codes, 64 bytes per group
+    uint8_t *s;       // scales, 4 bytes per group
+    int64_t rows, k, ld;
+    bool bf16;        // the plain side's type: bf16, or f32
+};
+hipError_t launch_mx_quantize(const MxCast &p, hipStream_t stream);
+hipError_t launch_mx_dequantize(const MxCast &p, hipStream_t stream);
+
+// y[m, n] = x[m, k] W[n, k]', W in MXFP4; x f32 (x != null) or MXFP4 (xq, xs).
+struct MxProblem {
+    const float *x;
+    const uint8_t *xq, *xs;
+    const uint8_t *wq, *ws;
+    float *y;
+    int64_t m, k, n;
+};
+// Which kernel, and what it needs; depends on the problem and the device alone.
+struct MxPlan {
+    int kind;        // 0: rows (f32 x, few activation rows), 1: tiles
+    int tiles;       // rows: 16-row weight tiles per workgroup
+    int64_t grid_x, grid_y;
+    size_t workspace_bytes;
+};
+MxPlan plan_mx(const MxProblem &p, int num_cus);
+hipError_t launch_mx(const MxProblem &p, const MxPlan &plan, void *workspace, hipStream_t stream);
+
+struct KvCache {
+    uint8_t *k, *v, *ks, *vs;
+    int64_t pages;
+    int heads, page, dim;
+};
+struct KvBatch {
+    const int32_t *table;   // [batch, width] page ids
+    int64_t width;
+    const int32_t *lens;    // [batch] tokens of each sequence, the new ones counted
+    const int32_t *starts;  // [batch + 1] first new token's row of each sequence
+    int batch, max_new, max_len;
+};
+struct KvAppend {
+    KvCache c;
+    KvBatch b;
+    const void *k, *v;      // new tokens' rows [heads][dim], ld elements apart
+    int64_t k_ld, v_ld;
+    bool bf16;
+};
+hipError_t launch_kv_append(const KvAppend &p, hipStream_t stream);
+
+struct KvAttend {
+    KvCache c;
+    KvBatch b;
+    const void *q;
+    void *out;              // rows [q_heads][dim], ld elements apart
+    int64_t q_ld, out_ld;
+    int q_heads, window;
+    float scale;
+    bool bf16;
+};
+struct KvPlan {
+    int kind;               // 0: few query rows, the tokens split; 1: tiles of query rows
+    int splits;             // workgroups along a sequence's tokens
+    int chunk;              // tokens of each
+    int64_t grid_x;
+    size_t workspace_bytes;
+};
+bool kv_dim_served(int64_t dim);
+KvPlan plan_kv(const KvAttend &p, int num_cus);
+hipError_t launch_kv_attend(const KvAttend &p, const KvPlan &plan, void *workspace, hipStream_t stream);
+
+}  // namespace dmc

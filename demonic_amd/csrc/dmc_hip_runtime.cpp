@@ -17,6 +17,7 @@
 //   * no CPU arithmetic anywhere: a device failure is reported (int entries)
 //     or fatal (the void drop-in entries), never silently recomputed.
 #include "../../include/dmc_hip.h"
+#include "decode_launch.h"
 #include "gemv_launch.h"
 #include "npz_ingress.h"
 #include "residency.h"
@@ -1355,6 +1356,183 @@ int32_t dmc_hip_bf16_transpose_2d(int64_t src_dev, int64_t dst_dev, int64_t m, i
                                               reinterpret_cast<uint16_t *>(dst_dev), m, n, ctx().stream);
     if (e != hipSuccess) return hip_fail(e, "transpose launch");
     return DMC_HIP_OK;
+}
+
+// ---- 4-bit weights (MXFP4) -------------------------------------------------------
+
+namespace {
+
+// Sizes that the MXFP4 kernels index with 32 bits within a row and over groups of rows.
+bool mx_dims(int64_t rows, int64_t k) {
+    return rows >= 0 && k >= 0 && rows <= INT32_MAX && k <= (1 << 27) &&
+           (k == 0 || rows <= ((int64_t)UINT32_MAX - 64) / dmc::mx_groups(k));
+}
+
+int mx_cast(bool quantise, int64_t plain, int64_t dtype, int64_t ld, int64_t q, int64_t s, int64_t rows, int64_t k) {
+    if (!mx_dims(rows, k)) return fail(DMC_HIP_EINVAL, "bad MXFP4 shape");
+    if (dtype != DMC_HIP_F32 && dtype != DMC_HIP_BF16) return fail(DMC_HIP_EINVAL, "bad element type");
+    if (ld == 0) ld = k;
+    if (ld < k) return fail(DMC_HIP_EINVAL, "row stride below the row length");
+    if (rows == 0 || k == 0) return DMC_HIP_OK;
+    if (!plain || !q || !s) return fail(DMC_HIP_EINVAL, "null pointer");
+    const bool bf = dtype == DMC_HIP_BF16;
+    if (q % 16 || s % 4 || plain % (bf ? 2 : 4)) return fail(DMC_HIP_EINVAL, "misaligned MXFP4 operand");
+    int rc = ensure_init();
+    if (rc) return rc;
+    dmc::MxCast p{};
+    p.src = reinterpret_cast<const void *>(quantise ? plain : q);
+    p.dst = reinterpret_cast<void *>(quantise ? q : plain);
+    p.q = reinterpret_cast<uint8_t *>(q);
+    p.s = reinterpret_cast<uint8_t *>(s);
+    p.rows = rows;
+    p.k = k;
+    p.ld = ld;
+    p.bf16 = bf;
+    const hipError_t e = quantise ? dmc::launch_mx_quantize(p, ctx().stream) : dmc::launch_mx_dequantize(p, ctx().stream);
+    return e == hipSuccess ? DMC_HIP_OK : hip_fail(e, "MXFP4 conversion launch");
+}
+
+int mx_product(int64_t x, int64_t xq, int64_t xs, int64_t wq, int64_t ws, int64_t y, int64_t m, int64_t k, int64_t n,
+               bool packed_x) {
+    if (!valid_dims(m, k, n) || !mx_dims(n, k) || !mx_dims(m, k)) return fail(DMC_HIP_EINVAL, "bad product shape");
+    if (m == 0 || n == 0) return DMC_HIP_OK;
+    if (!y || (k > 0 && (!wq || !ws || (packed_x ? !xq || !xs : !x)))) return fail(DMC_HIP_EINVAL, "null pointer");
+    if (y % 4 || wq % 16 || ws % 4 || x % 4 || xq % 16 || xs % 4)
+        return fail(DMC_HIP_EINVAL, "misaligned operand of an MXFP4 product");
+    int rc = ensure_init();
+    if (rc) return rc;
+    Ctx &c = ctx();
+    dmc::MxProblem p{};
+    p.x = reinterpret_cast<const float *>(packed_x ? 0 : x);
+    p.xq = reinterpret_cast<const uint8_t *>(xq);
+    p.xs = reinterpret_cast<const uint8_t *>(xs);
+    p.wq = reinterpret_cast<const uint8_t *>(wq);
+    p.ws = reinterpret_cast<const uint8_t *>(ws);
+    p.y = reinterpret_cast<float *>(y);
+    p.m = m;
+    p.k = k;
+    p.n = n;
+    const dmc::MxPlan pl = dmc::plan_mx(p, c.cus);
+    if ((rc = ensure_dev(c.ws, pl.workspace_bytes))) return rc;
+    const hipError_t e = dmc::launch_mx(p, pl, c.ws.p, c.stream);
+    return e == hipSuccess ? DMC_HIP_OK : hip_fail(e, "MXFP4 product launch");
+}
+
+}  // namespace
+
+int64_t dmc_hip_mxfp4_row_bytes(int64_t k) { return k < 0 ? 0 : dmc::mx_groups(k) * 64; }
+int64_t dmc_hip_mxfp4_row_scales(int64_t k) { return k < 0 ? 0 : dmc::mx_groups(k) * 4; }
+
+int32_t dmc_hip_mxfp4_quantize(int64_t src_dev, int64_t dtype, int64_t ld, int64_t q_dev, int64_t s_dev, int64_t rows,
+                               int64_t k) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    return mx_cast(true, src_dev, dtype, ld, q_dev, s_dev, rows, k);
+}
+
+int32_t dmc_hip_mxfp4_dequantize(int64_t q_dev, int64_t s_dev, int64_t dst_dev, int64_t dtype, int64_t ld,
+                                 int64_t rows, int64_t k) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    return mx_cast(false, dst_dev, dtype, ld, q_dev, s_dev, rows, k);
+}
+
+int32_t dmc_hip_gemv_mxfp4_rd(int64_t x_dev, int64_t wq_dev, int64_t ws_dev, int64_t y_dev, int64_t m, int64_t k,
+                              int64_t n) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    return mx_product(x_dev, 0, 0, wq_dev, ws_dev, y_dev, m, k, n, false);
+}
+
+int32_t dmc_hip_gemm_mxfp4(int64_t xq_dev, int64_t xs_dev, int64_t wq_dev, int64_t ws_dev, int64_t y_dev, int64_t m,
+                           int64_t k, int64_t n) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    return mx_product(0, xq_dev, xs_dev, wq_dev, ws_dev, y_dev, m, k, n, true);
+}
+
+// ---- the 8-bit attention cache -----------------------------------------------------
+
+namespace {
+
+int kv_args(const dmc_hip_kv8 *cache, const dmc_hip_kv8_batch *batch, int64_t dtype, dmc::KvCache &c, dmc::KvBatch &b) {
+    if (!cache || !batch) return fail(DMC_HIP_EINVAL, "null cache or batch");
+    if (dtype != DMC_HIP_F32 && dtype != DMC_HIP_BF16) return fail(DMC_HIP_EINVAL, "bad element type");
+    if (!dmc::kv_dim_served(cache->dim)) return fail(DMC_HIP_EINVAL, "head dim %lld: 64, 96, 128 and 256 are served", (long long)cache->dim);
+    if (cache->page != 16 && cache->page != 32 && cache->page != 64 && cache->page != 128 && cache->page != 256)
+        return fail(DMC_HIP_EINVAL, "page of %lld tokens: 16, 32, 64, 128 and 256 are served", (long long)cache->page);
+    if (cache->heads < 1 || cache->heads > 4096 || cache->pages < 1 || cache->pages > INT32_MAX)
+        return fail(DMC_HIP_EINVAL, "bad cache shape");
+    if (batch->batch < 0 || batch->batch > 32767 || batch->width < 0 || batch->width > INT32_MAX || batch->max_new < 0 ||
+        batch->max_new > (1 << 24) || batch->max_len < 0 || batch->max_len > (1 << 30))
+        return fail(DMC_HIP_EINVAL, "bad batch shape");
+    if (!cache->k_dev || !cache->v_dev || !cache->k_scales_dev || !cache->v_scales_dev)
+        return fail(DMC_HIP_EINVAL, "null cache pointer");
+    if (cache->k_dev % 16 || cache->v_dev % 16) return fail(DMC_HIP_EINVAL, "cache pages must be 16-byte aligned");
+    if (batch->batch > 0 && batch->max_new > 0) {
+        if (!batch->table_dev || !batch->lens_dev || !batch->starts_dev) return fail(DMC_HIP_EINVAL, "null batch pointer");
+        if (batch->table_dev % 4 || batch->lens_dev % 4 || batch->starts_dev % 4)
+            return fail(DMC_HIP_EINVAL, "misaligned batch pointer");
+    }
+    c = {reinterpret_cast<uint8_t *>(cache->k_dev), reinterpret_cast<uint8_t *>(cache->v_dev),
+         reinterpret_cast<uint8_t *>(cache->k_scales_dev), reinterpret_cast<uint8_t *>(cache->v_scales_dev), cache->pages,
+         (int)cache->heads, (int)cache->page, (int)cache->dim};
+    b = {reinterpret_cast<const int32_t *>(batch->table_dev), batch->width, reinterpret_cast<const int32_t *>(batch->lens_dev),
+         reinterpret_cast<const int32_t *>(batch->starts_dev), (int)batch->batch, (int)batch->max_new, (int)batch->max_len};
+    return DMC_HIP_OK;
+}
+
+// A row pointer and stride of a side with `heads` heads; 0 means packed.
+int kv_rows(int64_t p, int64_t &ld, int64_t heads, int64_t dim, bool bf) {
+    if (ld == 0) ld = heads * dim;
+    if (ld < heads * dim) return fail(DMC_HIP_EINVAL, "row stride below heads * dim");
+    if (!p) return fail(DMC_HIP_EINVAL, "null pointer");
+    if (p % (bf ? 2 : 4)) return fail(DMC_HIP_EINVAL, "misaligned rows");
+    return DMC_HIP_OK;
+}
+
+}  // namespace
+
+int32_t dmc_hip_kv8_append(const dmc_hip_kv8 *cache, const dmc_hip_kv8_batch *batch, int64_t k_dev, int64_t v_dev,
+                           int64_t dtype, int64_t k_ld, int64_t v_ld) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    dmc::KvAppend p{};
+    int rc = kv_args(cache, batch, dtype, p.c, p.b);
+    if (rc) return rc;
+    if (p.b.batch == 0 || p.b.max_new == 0) return DMC_HIP_OK;
+    p.bf16 = dtype == DMC_HIP_BF16;
+    if ((rc = kv_rows(k_dev, k_ld, p.c.heads, p.c.dim, p.bf16)) || (rc = kv_rows(v_dev, v_ld, p.c.heads, p.c.dim, p.bf16)))
+        return rc;
+    if ((rc = ensure_init())) return rc;
+    p.k = reinterpret_cast<const void *>(k_dev);
+    p.v = reinterpret_cast<const void *>(v_dev);
+    p.k_ld = k_ld;
+    p.v_ld = v_ld;
+    const hipError_t e = dmc::launch_kv_append(p, ctx().stream);
+    return e == hipSuccess ? DMC_HIP_OK : hip_fail(e, "cache append launch");
+}
+
+int32_t dmc_hip_kv8_attend(const dmc_hip_kv8 *cache, const dmc_hip_kv8_batch *batch, int64_t q_dev, int64_t out_dev,
+                           int64_t dtype, int64_t q_heads, int64_t q_ld, int64_t out_ld, float scale, int64_t window) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    dmc::KvAttend p{};
+    int rc = kv_args(cache, batch, dtype, p.c, p.b);
+    if (rc) return rc;
+    if (q_heads < 1 || q_heads > 65535 || q_heads % p.c.heads) return fail(DMC_HIP_EINVAL, "query heads must be a multiple of the cache's");
+    if (window < 0) return fail(DMC_HIP_EINVAL, "negative window");
+    if (p.b.batch == 0 || p.b.max_new == 0) return DMC_HIP_OK;
+    p.bf16 = dtype == DMC_HIP_BF16;
+    if ((rc = kv_rows(q_dev, q_ld, q_heads, p.c.dim, p.bf16)) || (rc = kv_rows(out_dev, out_ld, q_heads, p.c.dim, p.bf16)))
+        return rc;
+    if ((rc = ensure_init())) return rc;
+    Ctx &c = ctx();
+    p.q = reinterpret_cast<const void *>(q_dev);
+    p.out = reinterpret_cast<void *>(out_dev);
+    p.q_ld = q_ld;
+    p.out_ld = out_ld;
+    p.q_heads = (int)q_heads;
+    p.scale = scale;
+    p.window = (int)std::min<int64_t>(window, 1 << 30);
+    const dmc::KvPlan pl = dmc::plan_kv(p, c.cus);
+    if ((rc = ensure_dev(c.ws, pl.workspace_bytes))) return rc;
+    const hipError_t e = dmc::launch_kv_attend(p, pl, c.ws.p, c.stream);
+    return e == hipSuccess ? DMC_HIP_OK : hip_fail(e, "attention launch");
 }
 
 int32_t dmc_hip_capture_begin(void) {

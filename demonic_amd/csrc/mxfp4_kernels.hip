@@ -1,0 +1,575 @@
+// mxfp4_kernels.hip -- microscaled 4-bit floating point: quantisation, its
+// inverse, and the products with 4-bit weights.
+#include "decode_launch.h"
+#include "gemv_device.h"
+
+#include <algorithm>
+
+namespace dmc {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// ---- quantisation -------------------------------------------------------------
+//
+// A block of 32 values x becomes codes c and a scale 2^e:
+//   e = floor(log2(max |x|)) - 2, within [-127, 127]   (6 = 1.5 * 2^2 is the largest code)
+//   c = x / 2^e, to the nearest e2m1 value, ties to the even code, at most 6.
+// Dividing by a power of two is exact, so there is one rounding.  A block that
+// holds an inf or a NaN has no such scale: its byte is 255 and it reads as NaN.
+// floor(log2) is the exponent field: the largest magnitude is taken as an
+// integer, where infs and NaNs come out above every finite value.
+//
+// A lane takes 8 values (a quarter of a block; the maximum crosses 4 lanes by
+// DPP), 16 lanes a group of 128, whose 64 code bytes and 4 scale bytes leave as
+// one dword per lane and one per group.
+
+// The least E of a block, as its biased byte; amax = the bits of max |x|.
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax) {
+    const uint32_t e = amax >> 23;
+    return e == 255 ? 255u : (e > 2 ? e - 2 : 0u);
+}
+
+__device__ __forceinline__ uint32_t row_or(uint32_t v) {  // over lanes 0, 4, 8, 12 of each 16
+    v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false);  // row_ror:4
+    v |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false);  // row_ror:8
+    return v;
+}
+
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false));  // quad_perm 1,0,3,2
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));  // quad_perm 2,3,0,1
+    return v;
+}
+
+struct __attribute__((packed, aligned(4))) F32x8 { f32x4 a, b; };
+struct __attribute__((packed, aligned(2))) U16x8 { u32x4 a; };
+
+template <bool BF>
+struct MxIn {
+    uint32_t u[BF ? 4 : 8];
+    __device__ __forceinline__ void load(const void *src, int64_t at, int left) {
+        if (left >= 8) {
+            if constexpr (BF) {
+                const U16x8 t = *reinterpret_cast<const U16x8 *>(static_cast<const uint16_t *>(src) + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) u[i] = t.a[i];
+            } else {
+                const F32x8 t = *reinterpret_cast<const F32x8 *>(static_cast<const float *>(src) + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    u[i] = __float_as_uint(t.a[i]);
+                    u[4 + i] = __float_as_uint(t.b[i]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (BF) {
+                    const uint32_t v = i < left ? static_cast<const uint16_t *>(src)[at + i] : 0u;
+                    u[i >> 1] = (i & 1) ? u[i >> 1] | v << 16 : v;
+                } else {
+                    u[i] = i < left ? __float_as_uint(static_cast<const float *>(src)[at + i]) : 0u;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t amax() const {
+        uint32_t v = 0;
+#pragma unroll
+        for (int i = 0; i < (BF ? 4 : 8); ++i) {
+            if constexpr (BF) v = max(v, max((u[i] << 16) & 0x7fffffffu, u[i] & 0x7fff0000u));
+            else v = max(v, u[i] & 0x7fffffffu);
+        }
+        return v;
+    }
+    __device__ __forceinline__ uint32_t codes(uint32_t byte) const {
+        const float sc = __uint_as_float(byte << 23);  // the conversions read the exponent field alone
+        uint32_t r = 0;
+        if constexpr (BF) {
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2_t, u[0]), sc, 0);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2_t, u[1]), sc, 1);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2_t, u[2]), sc, 2);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2_t, u[3]), sc, 3);
+        } else {
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(u[0]), __uint_as_float(u[1]), sc, 0);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(u[2]), __uint_as_float(u[3]), sc, 1);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(u[4]), __uint_as_float(u[5]), sc, 2);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(u[6]), __uint_as_float(u[7]), sc, 3);
+        }
+        return byte == 255 ? 0u : r;
+    }
+};
+
+// Groups are numbered over all rows; lane 16 j + i of a wave has values 8 i .. 8 i + 7 of the wave's j-th.
+template <bool BF>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const void *__restrict__ src, uint32_t *__restrict__ q,
+                                                          uint32_t *__restrict__ s, uint32_t groups, uint32_t per_row,
+                                                          int k, int64_t ld) {
+    const uint32_t i = threadIdx.x & 15;
+    const uint32_t g = blockIdx.x * 16u + (threadIdx.x >> 4);
+    if (g >= groups) return;
+    const uint32_t row = g / per_row, at = (g - row * per_row) * 128u + 8u * i;
+    MxIn<BF> v;
+    v.load(src, (int64_t)row * ld + at, k - (int)at);
+    const uint32_t byte = mx_scale_byte(quad_max(v.amax()));
+    q[(uint64_t)g * 16 + i] = v.codes(byte);
+    const uint32_t sc = row_or((i & 3) == 0 ? byte << (2 * i) : 0u);
+    if (i == 0) s[g] = sc;
+}
+
+// The f32 bits of 2^(byte - 127); 255 is NaN, 0 is 2^-127, a subnormal.
+__device__ __forceinline__ float e8m0(uint32_t byte) {
+    return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
+}
+
+template <bool BF>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t *__restrict__ q,
+                                                            const uint8_t *__restrict__ s, void *__restrict__ dst,
+                                                            uint32_t groups, uint32_t per_row, int k, int64_t ld) {
+    const uint32_t i = threadIdx.x & 15;
+    const uint32_t g = blockIdx.x * 16u + (threadIdx.x >> 4);
+    if (g >= groups) return;
+    const uint32_t row = g / per_row, at = (g - row * per_row) * 128u + 8u * i;
+    const uint32_t c = q[(uint64_t)g * 16 + i];
+    const float sc = e8m0(s[(uint64_t)g * 4 + (i >> 2)]);
+    const int64_t o = (int64_t)row * ld + at;
+    const int left = k - (int)at;
+    // a code's value times its scale: exact in f32, and in bf16 but for a NaN's payload
+    f32x2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1),
+                  __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3)};
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = p[j >> 1][j & 1] * sc;
+    if constexpr (BF) {
+        uint16_t *d = static_cast<uint16_t *>(dst) + o;
+        if (left >= 8) {
+            U16x8 t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t.a[j] = (__float_as_uint(f[2 * j]) >> 16) | (__float_as_uint(f[2 * j + 1]) & 0xffff0000u);
+            *reinterpret_cast<U16x8 *>(d) = t;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < left) d[j] = (uint16_t)(__float_as_uint(f[j]) >> 16);
+        }
+    } else {
+        float *d = static_cast<float *>(dst) + o;
+        if (left >= 8) {
+            *reinterpret_cast<F32x8 *>(d) = F32x8{{f[0], f[1], f[2], f[3]}, {f[4], f[5], f[6], f[7]}};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < left) d[j] = f[j];
+        }
+    }
+}
+
+// ---- product, few activation rows ------------------------------------------------
+//
+// y = x W' with x f32 and at most 5 rows.  Each activation is the sum of three
+// bf16 terms (8 + 8 + 8 bits of its 24, cut, so the sum is exact); a code times
+// its scale is exact in bf16 too; so the matrix cores' products are exact and
+// only their f32 sums round.  The 3 m terms are columns of one 16-wide tile.
+//
+// A workgroup of 8 waves owns T tiles of 16 weight rows and walks k in chunks of
+// 4096: the terms of x go to LDS once per chunk, each wave takes 512 k of every
+// tile, and the waves' sums meet in LDS at the end, in wave order.
+constexpr int kRowsWaves = 8;
+constexpr int kRowsSteps = 4;                              // groups of 128 per wave and chunk
+constexpr int kRowsChunk = kRowsWaves * kRowsSteps * 128;  // 4096
+constexpr int kRowsMax = 5;                                // activation rows: 3 terms each in 16 columns
+constexpr int kRowsLds = kRowsChunk * 2 + 64;              // bytes of one term's chunk; 64 shift the banks
+
+__device__ __forceinline__ uint32_t cut2(float a, float b) {  // bf16 pair of two values' upper halves
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+
+struct MxStep {
+    u32x4 w;
+    uint32_t s;
+};
+
+template <int T>
+__global__ __launch_bounds__(512) void mx_rows_kernel(const float *__restrict__ x, const uint8_t *__restrict__ wq,
+                                                      const uint8_t *__restrict__ ws, float *__restrict__ y, int m,
+                                                      int k, int n) {
+    extern __shared__ char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = lane & 15, quad = lane >> 4;
+    const int groups = (k + 127) >> 7, cols = 3 * m;
+    const int64_t row0 = (int64_t)blockIdx.x * T * 16;
+    const int chunks = (groups + kRowsWaves * kRowsSteps - 1) / (kRowsWaves * kRowsSteps);
+    const uint32_t qrow = (uint32_t)groups * 64u, srow = (uint32_t)groups * 4u;
+
+    auto load = [&](MxStep *st, int t, int chunk) {
+        const int64_t at = row0 + t * 16;
+        const int64_t left = max((int64_t)0, min((int64_t)16, (int64_t)n - at));
+        const __amdgpu_buffer_rsrc_t qr = weight_rsrc(wq + at * qrow, (uint32_t)left * qrow);
+        const __amdgpu_buffer_rsrc_t sr = weight_rsrc(ws + at * srow, (uint32_t)left * srow);
+#pragma unroll
+        for (int i = 0; i < kRowsSteps; ++i) {
+            // past the row's end there is the next row: read as zeros instead
+            const int g = chunk * kRowsWaves * kRowsSteps + wave * kRowsSteps + i;
+            const uint32_t qo = g < groups ? (uint32_t)r * qrow + (uint32_t)g * 64u + quad * 16u : 0xfffffff0u;
+            const uint32_t so = g < groups ? (uint32_t)r * srow + (uint32_t)g * 4u : 0xfffffff0u;
+            st[i].w = load_w16(qr, qo);
+            st[i].s = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(sr, so, 0, kLoadNT);
+        }
+    };
+
+    f32x4 acc[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) acc[t] = f32x4{0, 0, 0, 0};
+    MxStep now[kRowsSteps];
+    load(now, 0, 0);
+    const char *xc = lds + min(r, cols - 1) * kRowsLds + wave * (kRowsSteps * 256) + quad * 64;
+    for (int c = 0; c < chunks; ++c) {
+        if (c) __syncthreads();
+        for (int i = threadIdx.x; i < m * (kRowsChunk / 8); i += 512) {
+            const int row = i / (kRowsChunk / 8), at = (i - row * (kRowsChunk / 8)) * 8;
+            const int k0 = c * kRowsChunk + at;
+            MxIn<false> v;
+            v.load(x, (int64_t)row * k + k0, max(0, k - k0));
+            u32x4 term[3];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float a[2], b[2], d[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t u = v.u[2 * j + h];
+                    const bool fin = (u & 0x7f800000u) != 0x7f800000u;
+                    // an inf or a NaN is its first term alone (a NaN kept one when cut)
+                    a[h] = __uint_as_float(fin ? u & 0xffff0000u : (u & 0x7fffffu) ? u | 0x400000u : u);
+                    const float r1 = __uint_as_float(u) - a[h];
+                    b[h] = fin ? __uint_as_float(__float_as_uint(r1) & 0xffff0000u) : 0.0f;
+                    d[h] = fin ? r1 - b[h] : 0.0f;
+                }
+                term[0][j] = cut2(a[0], a[1]);
+                term[1][j] = cut2(b[0], b[1]);
+                term[2][j] = cut2(d[0], d[1]);
+            }
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(lds + (row * 3 + p) * kRowsLds + at * 2) = term[p];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            // the next tile's weights (past the last chunk: zeros, unread)
+            MxStep next[kRowsSteps];
+            load(next, t < T - 1 ? t + 1 : 0, t < T - 1 ? c : c + 1);
+#pragma unroll
+            for (int i = 0; i < kRowsSteps; ++i) {
+                const float sc = e8m0((now[i].s >> (8 * quad)) & 255u);
+                const char *xb = xc + i * 256;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = now[i].w[j];
+                    u32x4 a;
+                    a[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
+                    a[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
+                    a[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
+                    a[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
+                    const u32x4 b = *reinterpret_cast<const u32x4 *>(xb + j * 16);
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                                     __builtin_bit_cast(bf16x8, b),
+                                                                     acc[t], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kRowsSteps; ++i) now[i] = next[i];
+        }
+    }
+    __syncthreads();
+    float *red = reinterpret_cast<float *>(lds);  // [T][wave][col][16 rows]
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+        *reinterpret_cast<f32x4 *>(red + ((t * kRowsWaves + wave) * 16 + r) * 16 + quad * 4) = acc[t];
+    __syncthreads();
+    for (int i = threadIdx.x; i < T * 16 * m; i += 512) {
+        const int a = i / (T * 16), o = i - a * (T * 16), t = o >> 4;
+        const int64_t row = row0 + o;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRowsWaves; ++w) {
+            const float *p = red + ((t * kRowsWaves + w) * 16 + 3 * a) * 16 + (o & 15);
+            sum += (p[32] + p[16]) + p[0];  // the small terms first
+        }
+        if (row < n) y[(int64_t)a * n + row] = sum;
+    }
+}
+
+size_t rows_lds(int tiles, int m) {
+    return std::max((size_t)3 * m * kRowsLds, (size_t)tiles * kRowsWaves * 16 * 16 * 4);
+}
+
+// ---- product, tiles ---------------------------------------------------------------
+//
+// The scaled MFMA takes both sides as they are stored: 16 x 16 outputs over 128 k,
+// lane 16 q + r holding block q of row r with that block's scale byte.
+//
+// x in MXFP4 is one such operand.  x in f32 is five: with amax < 2^(e+2) the
+// largest magnitude of a block, the whole number I = round(x 2^(22-e)) has at most
+// 25 bits with its sign, and is written in base 32 with digits of [-16, 16], each
+// of which is an e2m3 value (digit / 4).  Digit p then carries the scale
+// 2^(e - 5 p), and the five products add up to x's at 24 bits of the block's
+// largest value, as a sum in f32 of such products has them.
+//
+// The planes of x: for each group of 128 k, each 16 activation rows and each digit
+// 64 lanes x 24 bytes, and per group and 16 rows 64 x 8 bytes of scales (the
+// digits' bytes, the first first).  A row that holds an inf or a NaN is marked and
+// its outputs are summed product by product instead.
+constexpr int kDigits = 5;
+constexpr int kPlaneBytes = 64 * 24;
+
+size_t planes_bytes(int64_t m, int64_t k) { return (size_t)(mx_groups(k) * ((m + 15) / 16)) * (kDigits * kPlaneBytes + 512); }
+
+__global__ __launch_bounds__(256) void mx_split_kernel(const float *__restrict__ x, char *__restrict__ planes,
+                                                       u32x2 *__restrict__ scales, uint32_t *__restrict__ marks,
+                                                       int m, int k, int groups, int rtiles) {
+    // 4 lanes per block of 32: lane j has values 8 j .. 8 j + 7
+    const int j = threadIdx.x & 3;
+    const int64_t b = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 2;  // (group, row tile, lane)
+    const int64_t unit = b >> 6;
+    if (unit >= (int64_t)groups * rtiles) return;
+    const int lane = (int)(b & 63), g = (int)(unit / rtiles), rt = (int)(unit - (int64_t)g * rtiles);
+    const int row = rt * 16 + (lane & 15), at = g * 128 + (lane >> 4) * 32 + j * 8;
+    MxIn<false> v;
+    v.load(x, (int64_t)min(row, m - 1) * k + at, row < m ? max(0, k - at) : 0);
+    const uint32_t amax = quad_max(v.amax());
+    const bool bad = amax >= 0x7f800000u;
+    // the first digit's scale byte: amax in [2, 4) of it; 20 at least, so that the last digit's is one
+    const int base = max((int)(amax >> 23) - 1, 20);
+    if (bad && j == 0) atomicOr(&marks[row >> 5], 1u << (row & 31));
+    int num[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = ldexpf(__uint_as_float(v.u[i]), 149 - base);
+        num[i] = bad ? 0 : (int)rintf(f);
+    }
+    char *o = planes + unit * (kDigits * kPlaneBytes) + lane * 24 + j * 6;
+#pragma unroll
+    for (int p = kDigits - 1; p >= 0; --p) {
+        uint64_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int d = p ? ((num[i] + 16) & 31) - 16 : num[i];
+            num[i] = (num[i] - d) >> 5;
+            const uint32_t a = (uint32_t)abs(d);
+            // e2m3 of a / 4: eighths below 2, quarters from there
+            bits |= (uint64_t)((a + min(a, 8u)) | (d < 0 ? 32u : 0u)) << (6 * i);
+        }
+        uint16_t *w = reinterpret_cast<uint16_t *>(o + p * kPlaneBytes);
+        w[0] = (uint16_t)bits;
+        w[1] = (uint16_t)(bits >> 16);
+        w[2] = (uint16_t)(bits >> 32);
+    }
+    if (j == 0) {
+        const uint32_t s = (uint32_t)base;
+        scales[unit * 64 + lane] = u32x2{s | (s - 5) << 8 | (s - 10) << 16 | (s - 15) << 24, s - 20};
+    }
+}
+
+// One output of a marked row, product by product.
+__device__ float mx_plain_dot(const float *x, const uint8_t *wq, const uint8_t *ws, int k) {
+    float sum = 0.0f;
+    for (int i = 0; i < k; ++i) {
+        const uint32_t c = (wq[i >> 1] >> (4 * (i & 1))) & 15u, mag = c & 7u;
+        const float v = mag < 2 ? 0.5f * (float)mag : ldexpf(1.0f + 0.5f * (float)(mag & 1), (int)(mag >> 1) - 1);
+        sum = fmaf(x[i], (c & 8u ? -v : v) * e8m0(ws[i >> 5]), sum);
+    }
+    return sum;
+}
+
+struct MxTileArgs {
+    const float *x;
+    const uint8_t *xq, *xs, *wq, *ws;
+    const char *planes;
+    const u32x2 *scales;
+    const uint32_t *marks;
+    float *y;
+    int m, k, n, groups, rtiles;
+};
+
+template <int PL, int RT, int CT>
+__global__ __launch_bounds__(256) void mx_tile_kernel(const MxTileArgs p) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = lane & 15, quad = lane >> 4;
+    const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * RT * 16;
+    const int m0 = blockIdx.y * CT * 16;
+    if (n0 >= p.n) return;
+    const int64_t qrow = (int64_t)p.groups * 64, srow = (int64_t)p.groups * 4;
+    const uint8_t *wq[RT], *ws[RT], *xq[CT], *xs[CT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        const int64_t row = min(n0 + i * 16 + r, (int64_t)p.n - 1);
+        wq[i] = p.wq + row * qrow + quad * 16;
+        ws[i] = p.ws + row * srow + quad;
+    }
+#pragma unroll
+    for (int i = 0; i < CT; ++i) {
+        const int64_t row = min(m0 + i * 16 + r, p.m - 1);
+        xq[i] = PL == 1 ? p.xq + row * qrow + quad * 16 : nullptr;
+        xs[i] = PL == 1 ? p.xs + row * srow + quad : nullptr;
+    }
+    f32x4 acc[RT][CT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    for (int g = 0; g < p.groups; ++g) {
+        i32x8 a[RT];
+        int as[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const u32x4 t = *reinterpret_cast<const u32x4 *>(wq[i] + (int64_t)g * 64);
+            a[i] = i32x8{(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
+            as[i] = ws[i][(int64_t)g * 4];
+        }
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            if constexpr (PL == 1) {
+                const u32x4 t = *reinterpret_cast<const u32x4 *>(xq[j] + (int64_t)g * 64);
+                const i32x8 b = {(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
+                const int bs = xs[j][(int64_t)g * 4];
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 4, 0, as[i], 0, bs);
+            } else {
+                const int64_t unit = (int64_t)g * p.rtiles + min((m0 >> 4) + j, p.rtiles - 1);
+                const u32x2 sc = p.scales[unit * 64 + lane];
+                const char *pb = p.planes + unit * (PL * kPlaneBytes) + lane * 24;
+#define DMC_DIGIT(P, SEL, WORD)                                                                                     \
+    {                                                                                                               \
+        const u32x2 *t = reinterpret_cast<const u32x2 *>(pb + P * kPlaneBytes);                                     \
+        const u32x2 t0 = t[0], t1 = t[1], t2 = t[2];                                                                \
+        const i32x8 b = {(int)t0[0], (int)t0[1], (int)t1[0], (int)t1[1], (int)t2[0], (int)t2[1], 0, 0};             \
+        _Pragma("unroll") for (int i = 0; i < RT; ++i) acc[i][j] =                                                  \
+            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 2, 0, as[i], SEL, (int)sc[WORD]); \
+    }
+                DMC_DIGIT(4, 0, 1)
+                DMC_DIGIT(3, 3, 0)
+                DMC_DIGIT(2, 2, 0)
+                DMC_DIGIT(1, 1, 0)
+                DMC_DIGIT(0, 0, 0)
+#undef DMC_DIGIT
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < CT; ++j) {
+        const int col = m0 + j * 16 + r;
+        if (col >= p.m) continue;
+        const bool marked = PL > 1 && (p.marks[col >> 5] >> (col & 31) & 1u);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int64_t row = n0 + i * 16 + quad * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (row + e >= p.n) continue;
+                float v = acc[i][j][e];
+                if (marked)
+                    v = mx_plain_dot(p.x + (int64_t)col * p.k, p.wq + (row + e) * qrow, p.ws + (row + e) * srow, p.k);
+                p.y[(int64_t)col * p.n + row + e] = v;
+            }
+        }
+    }
+}
+
+__global__ void mx_clear_kernel(uint32_t *p, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 0;
+}
+
+__global__ void mx_zero_kernel(float *y, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) y[i] = 0.0f;
+}
+
+int div_up(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+}  // namespace
+
+hipError_t launch_mx_quantize(const MxCast &p, hipStream_t stream) {
+    const uint32_t per = (uint32_t)mx_groups(p.k), groups = (uint32_t)p.rows * per;
+    auto f = p.bf16 ? mx_quantize_kernel<true> : mx_quantize_kernel<false>;
+    f<<<dim3((groups + 15) / 16), dim3(256), 0, stream>>>(p.src, reinterpret_cast<uint32_t *>(p.q),
+                                                          reinterpret_cast<uint32_t *>(p.s), groups, per, (int)p.k, p.ld);
+    return hipGetLastError();
+}
+
+hipError_t launch_mx_dequantize(const MxCast &p, hipStream_t stream) {
+    const uint32_t per = (uint32_t)mx_groups(p.k), groups = (uint32_t)p.rows * per;
+    auto f = p.bf16 ? mx_dequantize_kernel<true> : mx_dequantize_kernel<false>;
+    f<<<dim3((groups + 15) / 16), dim3(256), 0, stream>>>(reinterpret_cast<const uint32_t *>(p.q), p.s, p.dst, groups,
+                                                          per, (int)p.k, p.ld);
+    return hipGetLastError();
+}
+
+MxPlan plan_mx(const MxProblem &p, int num_cus) {
+    MxPlan pl{};
+    if (p.k == 0) return pl;
+    if (p.x && p.m <= kRowsMax) {
+        pl.kind = 0;
+        const int64_t tiles = (p.n + 15) / 16;
+        pl.tiles = tiles >= 8 * 4 * (int64_t)num_cus ? 8 : tiles >= 2 * 4 * (int64_t)num_cus ? 2 : 1;
+        pl.grid_x = (tiles + pl.tiles - 1) / pl.tiles;
+        pl.grid_y = 1;
+    } else {
+        pl.kind = 1;
+        pl.grid_x = div_up(p.n, 4 * 2 * 16);
+        pl.grid_y = div_up(p.m, 2 * 16);
+        if (p.x) pl.workspace_bytes = planes_bytes(p.m, p.k) + (size_t)((p.m + 31) / 32) * 4;
+    }
+    return pl;
+}
+
+hipError_t launch_mx(const MxProblem &p, const MxPlan &pl, void *workspace, hipStream_t stream) {
+    if (p.k == 0) {
+        mx_zero_kernel<<<dim3((unsigned)std::min<int64_t>(4096, (p.m * p.n + 255) / 256)), dim3(256), 0, stream>>>(p.y, p.m * p.n);
+        return hipGetLastError();
+    }
+    if (pl.kind == 0) {
+        const size_t lds = rows_lds(pl.tiles, (int)p.m);
+        auto f = pl.tiles == 8 ? mx_rows_kernel<8> : pl.tiles == 2 ? mx_rows_kernel<2> : mx_rows_kernel<1>;
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        if (e != hipSuccess) return e;
+        f<<<dim3((unsigned)pl.grid_x), dim3(512), lds, stream>>>(p.x, p.wq, p.ws, p.y, (int)p.m, (int)p.k, (int)p.n);
+        return hipGetLastError();
+    }
+    MxTileArgs a{};
+    a.x = p.x;
+    a.xq = p.xq;
+    a.xs = p.xs;
+    a.wq = p.wq;
+    a.ws = p.ws;
+    a.y = p.y;
+    a.m = (int)p.m;
+    a.k = (int)p.k;
+    a.n = (int)p.n;
+    a.groups = (int)mx_groups(p.k);
+    a.rtiles = div_up(p.m, 16);
+    const dim3 grid((unsigned)pl.grid_x, (unsigned)pl.grid_y);
+    if (p.x) {
+        const int64_t units = (int64_t)a.groups * a.rtiles;
+        char *w = static_cast<char *>(workspace);
+        char *planes = w;
+        u32x2 *scales = reinterpret_cast<u32x2 *>(w + units * kDigits * kPlaneBytes);
+        uint32_t *marks = reinterpret_cast<uint32_t *>(w + units * (kDigits * kPlaneBytes + 512));
+        const int words = div_up(p.m, 32);
+        mx_clear_kernel<<<dim3(div_up(words, 256)), dim3(256), 0, stream>>>(marks, words);
+        mx_split_kernel<<<dim3((unsigned)units), dim3(256), 0, stream>>>(p.x, planes, scales, marks, a.m, a.k, a.groups, a.rtiles);
+        a.planes = planes;
+        a.scales = scales;
+        a.marks = marks;
+        mx_tile_kernel<kDigits, 2, 2><<<grid, dim3(256), 0, stream>>>(a);
+    } else {
+        mx_tile_kernel<1, 2, 2><<<grid, dim3(256), 0, stream>>>(a);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace dmc

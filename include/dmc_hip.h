@@ -281,6 +281,90 @@ int32_t dmc_hip_bf16_upconvert(int64_t src_dev, int64_t dst_dev, int64_t n);
 int32_t dmc_hip_f32_to_bf16(int64_t src_dev, int64_t dst_dev, int64_t n);
 int32_t dmc_hip_bf16_transpose_2d(int64_t src_dev, int64_t dst_dev, int64_t m, int64_t n);
 
+/* ---- 4-bit weights: MXFP4 -------------------------------------------------
+ *
+ * No counterpart in the reference.  A row of k values is ceil(k / 128) groups of
+ * 128; each group is 64 bytes of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+ * their negatives; two to a byte, the first in the low half) and 4 scale bytes,
+ * one per block of 32: a code stands for code * 2^(byte - 127), and byte 255
+ * makes its block NaN.  Rows lie dmc_hip_mxfp4_row_bytes(k) and
+ * dmc_hip_mxfp4_row_scales(k) bytes apart; what lies past k in a row's last group
+ * is code 0 (the quantiser writes it so, and the products rely on it).  Codes are
+ * 16-byte aligned, scales 4-byte aligned.  All entries are on device pointers,
+ * ordered on the library stream, and may be recorded into a graph. */
+#define DMC_HIP_F32 0
+#define DMC_HIP_BF16 1
+int64_t dmc_hip_mxfp4_row_bytes(int64_t k);
+int64_t dmc_hip_mxfp4_row_scales(int64_t k);
+
+/* rows [rows][k] (ld elements apart, 0: k; f32 or bf16 by dtype) to MXFP4: scale
+ * 2^e, e = floor(log2(max |x|)) - 2 within [-127, 127] for each block of 32, codes
+ * x / 2^e to the nearest, ties to the even code, at most 6 in magnitude.  A block
+ * that holds an inf or a NaN gets byte 255 and codes 0.  The inverse writes the
+ * values that the codes stand for: exact in f32 and in bf16. */
+int32_t dmc_hip_mxfp4_quantize(int64_t src_dev, int64_t dtype, int64_t ld, int64_t q_dev, int64_t s_dev,
+                               int64_t rows, int64_t k);
+int32_t dmc_hip_mxfp4_dequantize(int64_t q_dev, int64_t s_dev, int64_t dst_dev, int64_t dtype, int64_t ld,
+                                 int64_t rows, int64_t k);
+
+/* y f32 [m,n] = x f32 [m,k] @ W', W [n,k] in MXFP4: dmc_hip_gemv_rd's product on
+ * 4-bit weights, any m.  x enters with its 24 bits (of its block of 32's largest
+ * value from 6 rows on), products are exact, sums are f32; NaN and inf classes are
+ * the formula's.  k == 0 writes +0.0.  From 6 rows on x's digits take a workspace
+ * of ceil(m / 16) * ceil(k / 128) * 8192 bytes plus 4 per 32 rows. */
+int32_t dmc_hip_gemv_mxfp4_rd(int64_t x_dev, int64_t wq_dev, int64_t ws_dev, int64_t y_dev, int64_t m,
+                              int64_t k, int64_t n);
+
+/* y f32 [m,n] = X @ W' with both in MXFP4 (X [m,k] as the quantiser writes it). */
+int32_t dmc_hip_gemm_mxfp4(int64_t xq_dev, int64_t xs_dev, int64_t wq_dev, int64_t ws_dev, int64_t y_dev,
+                           int64_t m, int64_t k, int64_t n);
+
+/* ---- the 8-bit attention cache ----------------------------------------------
+ *
+ * No counterpart in the reference.  A pool of `pages` pages; a page holds `page`
+ * (16, 32, 64, 128 or 256) tokens of `heads` heads of `dim` (64, 96, 128 or 256)
+ * values in e4m3, K as [heads][page][dim] and V as [heads][dim][page], and one scale
+ * byte per page, head and side ([pages][heads]): a code stands for
+ * code * 2^(byte - 127).  Pages are 16-byte aligned.
+ *
+ * A batch describes sequences, on the device: the page ids of each one's tokens
+ * (table int32 [batch][width]; an id outside [0, pages) is a page that is not
+ * there: its tokens are not stored and not seen), its tokens, the new ones counted
+ * (lens int32 [batch]), and where its new tokens' rows begin (starts int32
+ * [batch + 1], the last one the number of rows).  New token i of n is at position
+ * len - n + i.  max_new bounds every n; a sequence's new tokens past it are left out.
+ * max_len is the longest length, which splits the work (a longer sequence is still
+ * served whole). */
+typedef struct dmc_hip_kv8 {
+    int64_t k_dev, v_dev, k_scales_dev, v_scales_dev;
+    int64_t pages, heads, page, dim;
+} dmc_hip_kv8;
+typedef struct dmc_hip_kv8_batch {
+    int64_t table_dev, width, lens_dev, starts_dev;
+    int64_t batch, max_new, max_len;
+} dmc_hip_kv8_batch;
+
+/* Store the new tokens' k and v rows ([heads][dim], ld elements apart, 0: packed;
+ * f32 or bf16).  A page that had no earlier token of the sequence takes the least
+ * scale 2^e with max |x| <= 448 * 2^e; one that had keeps its scale or raises it
+ * to that, and then its earlier codes are rounded to the new scale.  Codes are
+ * x / 2^e to the nearest even; infs and NaNs are stored as NaN and do not enter
+ * the scale.  Sequences that append must not share the page they append to.  A
+ * sequence with len < n is left alone. */
+int32_t dmc_hip_kv8_append(const dmc_hip_kv8 *cache, const dmc_hip_kv8_batch *batch, int64_t k_dev, int64_t v_dev,
+                           int64_t dtype, int64_t k_ld, int64_t v_ld);
+
+/* out = softmax(scale * q K') V for each new token's rows (q_heads heads, a multiple
+ * of `heads`; q head h reads cache head h / (q_heads / heads)), over the tokens at
+ * positions t - window + 1 .. t (window 0: 0 .. t) of its own position t.  A row
+ * that sees nothing is 0.  Scores, weights, maxima and sums are f32; with f32 rows
+ * q and the weights enter the products with all their bits, with bf16 rows the
+ * weights are rounded to bf16.  Masked tokens have no effect, whatever their bits.
+ * The partial results of split sequences use the library workspace. */
+int32_t dmc_hip_kv8_attend(const dmc_hip_kv8 *cache, const dmc_hip_kv8_batch *batch, int64_t q_dev, int64_t out_dev,
+                           int64_t dtype, int64_t q_heads, int64_t q_ld, int64_t out_ld, float scale,
+                           int64_t window);
+
 /* HIP graphs of the library stream.  Between capture_begin and capture_end,
  * device-pointer GEMVs (dmc_hip_gemv_rd, _gemv_rd_grouped, _gemv_cs) are
  * recorded instead of run, provided that any plan whose dmc_hip_plan

@@ -1,0 +1,121 @@
+"""MXFP4 and the 8-bit cache on the CPU: the plain forms' own pins, and what the entries refuse before a device."""
+import numpy as np
+import pytest
+
+import demonic_amd as d
+import lowbits as L
+
+
+def test_mxfp4_rows():
+    assert [d.mxfp4_row(k) for k in (0, 1, 128, 129, 4096)] == [(0, 0), (64, 4), (64, 4), (128, 8), (2048, 128)]
+
+
+def test_plain_quantiser_rounds_to_nearest_even_and_saturates():
+    x = np.zeros((1, 32), np.float32)
+    x[0, :14] = [4, .25, .75, 1.25, 1.75, 2.5, 3.5, 5, 7.9, -.25, -5, .26, 2.51, 5.01]
+    q, s = L.mx_quantize(x)
+    assert s[0, 0] == 127
+    np.testing.assert_array_equal(L.mx_values(q, s, 14)[0], [4, 0, 1, 1, 2, 2, 4, 4, 6, -0., -4, .5, 3, 6])
+
+
+def test_plain_e4m3_matches_torch():
+    torch = pytest.importorskip("torch")
+    codes = np.arange(256, dtype=np.uint8)
+    t = torch.from_numpy(codes).view(torch.float8_e4m3fn).float().numpy()
+    np.testing.assert_array_equal(np.isnan(t), np.isnan(L.E4M3))
+    np.testing.assert_array_equal(t[~np.isnan(t)], L.E4M3[~np.isnan(t)])
+    x = np.random.default_rng(0).standard_normal(4096).astype(np.float32) * 60
+    x[:64] = np.float32(2.0) ** -10 * np.arange(64)
+    got = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    np.testing.assert_array_equal(L.e4m3_codes(x.astype(np.float64)), got)
+
+
+def test_plain_cache_scale_is_the_least():
+    assert L.cache_scale(np.array([448.0])) == 127 and L.cache_scale(np.array([448.1])) == 128
+    assert L.cache_scale(np.array([0.0, np.inf, np.nan])) == 0 and L.cache_scale(np.array([224.0])) == 126
+
+
+P = 1 << 12  # an address that no call gets to use
+
+
+@pytest.mark.parametrize("call", [
+    lambda: d.mxfp4_quantize(P, P, P, -1, 4),
+    lambda: d.mxfp4_quantize(P, P, P, 4, -1),
+    lambda: d.mxfp4_quantize(P, P, P, 4, 8, ld=7),
+    lambda: d.mxfp4_quantize(0, P, P, 4, 8),
+    lambda: d.mxfp4_quantize(P, P + 8, P, 4, 8),
+    lambda: d.mxfp4_quantize(P + 1, P, P, 4, 8, dtype="bf16"),
+    lambda: d.mxfp4_quantize(P + 2, P, P, 4, 8),
+    lambda: d.mxfp4_quantize(P, P, P, 1 << 31, 8),
+    lambda: d.mxfp4_quantize(P, P, P, 1 << 30, 1 << 20),
+    lambda: d.mxfp4_dequantize(P, P + 1, P, 4, 8),
+    lambda: d.mxfp4_dequantize(P, 0, P, 4, 8),
+    lambda: d.gemv_mxfp4_rd(P, P, P, P, -1, 8, 8),
+    lambda: d.gemv_mxfp4_rd(P, P, P, 0, 1, 8, 8),
+    lambda: d.gemv_mxfp4_rd(0, P, P, P, 1, 8, 8),
+    lambda: d.gemv_mxfp4_rd(P, P + 4, P, P, 1, 8, 8),
+    lambda: d.gemv_mxfp4_rd(P + 1, P, P, P, 1, 8, 8),
+    lambda: d.gemv_mxfp4_rd(P, P, P, P, 1, 1 << 28, 8),
+    lambda: d.gemm_mxfp4(P, 0, P, P, P, 1, 8, 8),
+    lambda: d.gemm_mxfp4(P + 8, P, P, P, P, 1, 8, 8),
+])
+def test_mxfp4_entries_refuse(call):
+    with pytest.raises(d.HipError) as e:
+        call()
+    assert e.value.code == -2 and str(e.value)
+
+
+def test_unknown_types_are_refused():
+    with pytest.raises(ValueError):
+        d.mxfp4_quantize(P, P, P, 1, 32, dtype="f16")
+    assert d._lib.load().dmc_hip_mxfp4_quantize(P, 2, 0, P, P, 1, 32) == -2
+
+
+def cache(**kw):
+    return d.KV8Cache(**{**dict(k=P, v=P, k_scales=P, v_scales=P, pages=4, heads=2, page=16, dim=64), **kw})
+
+
+def batch(**kw):
+    return d.KV8Batch(**{**dict(table=P, width=2, lens=P, starts=P, batch=1, max_new=1, max_len=32), **kw})
+
+
+BAD = [(cache(**c), batch(**b)) for c, b in (
+    [({n: v}, {}) for n, v in (("k", 0), ("v", 0), ("k_scales", 0), ("v_scales", 0), ("k", P + 8), ("v", P + 4), ("pages", 0),
+                               ("heads", 0), ("heads", 5000), ("page", 8), ("page", 48), ("page", 512), ("dim", 80), ("dim", 0))]
+    + [({}, {n: v}) for n, v in (("table", 0), ("lens", 0), ("starts", 0), ("table", P + 2), ("width", -1), ("batch", -1),
+                                 ("batch", 40000), ("max_new", -1), ("max_len", -1))])]
+
+
+@pytest.mark.parametrize("c,b", BAD, ids=[str(i) for i in range(len(BAD))])
+def test_cache_entries_refuse(c, b):
+    for call in (lambda: d.kv8_append(c, b, P, P), lambda: d.kv8_attend(c, b, P, P, 2)):
+        with pytest.raises(d.HipError) as e:
+            call()
+        assert e.value.code == -2 and str(e.value)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: d.kv8_append(cache(), batch(), 0, P),
+    lambda: d.kv8_append(cache(), batch(), P, P, k_ld=127),
+    lambda: d.kv8_append(cache(), batch(), P + 2, P),
+    lambda: d.kv8_append(cache(), batch(), P + 1, P, dtype="bf16"),
+    lambda: d.kv8_attend(cache(), batch(), P, 0, 2),
+    lambda: d.kv8_attend(cache(), batch(), P, P, 3),
+    lambda: d.kv8_attend(cache(), batch(), P, P, 0),
+    lambda: d.kv8_attend(cache(), batch(), P, P, 4, window=-1),
+    lambda: d.kv8_attend(cache(), batch(), P, P, 4, q_ld=255),
+    lambda: d.kv8_attend(cache(), batch(), P, P, 4, out_ld=1),
+])
+def test_cache_calls_refuse(call):
+    with pytest.raises(d.HipError) as e:
+        call()
+    assert e.value.code == -2
+
+
+def test_empty_calls_do_nothing_without_a_device():
+    d.mxfp4_quantize(0, 0, 0, 0, 64)
+    d.mxfp4_dequantize(0, 0, 0, 5, 0)
+    d.gemv_mxfp4_rd(0, 0, 0, 0, 0, 64, 8)
+    d.gemm_mxfp4(0, 0, 0, 0, 0, 3, 64, 0)
+    d.kv8_append(cache(), batch(batch=0, table=0, lens=0, starts=0), 0, 0)
+    d.kv8_attend(cache(), batch(max_new=0), 0, 0, 2)
