@@ -176,24 +176,53 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {
     return (((v & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
 }
 
+// Which of a lane's values of a column (dim 16 d + 4 quad + i is bit 4 d + i) meet a NaN code among the
+// tokens [lo, hi) that the column's row sees.  For the steps that some rows see in part: there a weight of
+// zero must not meet a NaN, so NaN codes are taken out of the products, and only if there were any is this
+// asked, once, at the end.
+__device__ __forceinline__ uint64_t nan_dims(const KvAttend &p, const int32_t *table, int head, int quad, int lo, int hi) {
+    uint64_t bits = 0;
+    const int P = p.c.page, D = p.c.dim, lgp = 31 - __clz(P);
+#pragma unroll 1
+    for (int n = 0; n < D / 4; ++n) {
+        const int dim = (n >> 2) * 16 + quad * 4 + (n & 3);
+#pragma unroll 1
+        for (int t = lo; t < hi; ++t) {
+            const int64_t id = table[t >> lgp];
+            if (id < 0 || id >= p.c.pages) continue;
+            if ((p.c.v[((id * p.c.heads + head) * D + dim) * P + (t & (P - 1))] & 0x7f) == 0x7f) bits |= 1ull << n;
+        }
+    }
+    return bits;
+}
+
+__device__ __forceinline__ float quads_max(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 struct KvPart {
     float *o;  // [splits][rows][dim]
     float *ml; // [splits][rows][2]
 };
 
-// Workgroups (column tile, token split), heads, sequences; 4 waves take steps of 64 tokens in turn.
+// Workgroups (column tile, token split), heads, sequences; 4 waves take steps of 64 tokens in turn, each
+// with the next step's codes on their way to registers while it works on this one's.
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const KvPart part, int splits, int chunk,
                                                       int row_tiles, int64_t rows_total) {
     constexpr int R = BF ? 16 : 4;      // query rows per column tile
     constexpr int KS = D / 32;          // MFMA steps over dims
     constexpr int DT = D / 16;          // tiles of dims
-    constexpr int LB = D / 4;           // dims of a lane of a K row
+    constexpr bool WIDE = KS % 2 == 0;  // K rows in 16-byte pieces (piece i of quad q: dims 64 i + 16 q on), else in 8
+    constexpr int KP = WIDE ? KS / 2 : KS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, quad = lane >> 4;
     const int split = blockIdx.x / row_tiles, tile = blockIdx.x - split * row_tiles;
     const int head = blockIdx.y, b = blockIdx.z;
-    const int group = p.q_heads / p.c.heads, P = p.c.page;
+    const int group = p.q_heads / p.c.heads, P = p.c.page, lgp = 31 - __clz(P);
     const int64_t start = p.b.starts[b];
     const int count = (int)min((int64_t)p.b.starts[b + 1] - start, (int64_t)p.b.max_new);
     const int row0 = tile * R, rows = count * group;  // query rows of this head: token row / group, head row % group
@@ -215,10 +244,50 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
     const int vis_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0, vis_hi = min(pos + 1, most);
     const int term = BF ? 0 : col >> 2;
 
+    const int32_t *table = p.b.table + (int64_t)b * p.b.width;
+    const float scale = p.scale * kLog2e;
+    const int64_t page_bytes = (int64_t)P * D;
+    auto page_of = [&](int t) -> int { return t < most ? table[t >> lgp] : -1; };
+    auto safe = [&](int id) -> int64_t { return id >= 0 && id < p.c.pages ? id : 0; };
+    struct Codes {
+        u32x4 v[DT];
+        u32x4 k[WIDE ? 4 * KP : 1];
+        u32x2 k8[WIDE ? 1 : 4 * KP];
+        uint32_t ks, vs;
+        bool in;
+    };
+    // the pages of the 16 tokens that a K row (its r / 4) and this lane's own tokens lie in
+    auto load = [&](Codes &c, int t0, int pk, int pv) {
+        const int tk = t0 + 16 * (col >> 2), tv = t0 + 16 * quad;
+        const uint8_t *kp = p.c.k + (safe(pk) * p.c.heads + head) * page_bytes + ((tk & (P - 1)) + (col & 3)) * D;
+        const uint8_t *vp = p.c.v + (safe(pv) * p.c.heads + head) * page_bytes + col * P + (tv & (P - 1));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                if constexpr (WIDE) c.k[j * KP + i] = *reinterpret_cast<const u32x4 *>(kp + j * 4 * D + i * 64 + quad * 16);
+                else c.k8[j * KP + i] = *reinterpret_cast<const u32x2 *>(kp + j * 4 * D + i * 32 + quad * 8);
+            }
+        c.ks = p.c.ks[safe(pv) * p.c.heads + head];
+        c.vs = p.c.vs[safe(pv) * p.c.heads + head];
+        c.in = pv >= 0 && pv < p.c.pages;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) c.v[d] = *reinterpret_cast<const u32x4 *>(vp + d * 16 * P);
+    };
+    Codes now;
+    int pk, pv;
+    {
+        const int t0 = from + wave * kStep;
+        load(now, t0, page_of(t0 + 16 * (col >> 2)), page_of(t0 + 16 * quad));
+        pk = page_of(t0 + 4 * kStep + 16 * (col >> 2));
+        pv = page_of(t0 + 4 * kStep + 16 * quad);
+    }
+
     u32x4 qf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        const int64_t at = tok * p.q_ld + (int64_t)qh * D + quad * LB + s * 8;
+        const int dim = WIDE ? (s >> 1) * 64 + quad * 16 + (s & 1) * 8 : s * 32 + quad * 8;
+        const int64_t at = tok * p.q_ld + (int64_t)qh * D + dim;
         if constexpr (BF) {
             struct __attribute__((packed, aligned(2))) T8 { u32x4 v; };
             qf[s] = reinterpret_cast<const T8 *>(static_cast<const uint16_t *>(p.q) + at)->v;
@@ -233,48 +302,73 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, sum = 0.0f;
-    const int32_t *table = p.b.table + (int64_t)b * p.b.width;
-    const float scale = p.scale * kLog2e;
-    const int64_t page_bytes = (int64_t)P * D;
+    uint32_t nans = 0;
 
     for (int t0 = from + wave * kStep; t0 < to; t0 += 4 * kStep) {
-        // the page of 16 tokens, for a K row (r / 4 of 4) and for this lane's own tokens
-        const int tk = t0 + 16 * (col >> 2), tv = t0 + 16 * quad;
-        const int64_t pk_raw = tk < most ? table[tk / P] : -1, pv_raw = tv < most ? table[tv / P] : -1;
-        const bool in_v = pv_raw >= 0 && pv_raw < p.c.pages;
-        const int64_t pk = pk_raw >= 0 && pk_raw < p.c.pages ? pk_raw : 0, pv = in_v ? pv_raw : 0;
-        const uint8_t *kp = p.c.k + (pk * p.c.heads + head) * page_bytes + (int64_t)(tk % P + (col & 3)) * D + quad * LB;
-        const uint8_t *vp = p.c.v + (pv * p.c.heads + head) * page_bytes + (int64_t)col * P + tv % P;
-        const float ks = e8m0(p.c.ks[pv * p.c.heads + head]) * scale, vs = e8m0(p.c.vs[pv * p.c.heads + head]);
+        Codes next;
+        load(next, t0 + 4 * kStep, pk, pv);  // past the end: some page's codes, not used
+        pk = page_of(t0 + 8 * kStep + 16 * (col >> 2));
+        pv = page_of(t0 + 8 * kStep + 16 * quad);
+        const int tv = t0 + 16 * quad;
+        const float ks = e8m0(now.ks) * scale, vs = e8m0(now.vs);
         float s[16];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            u32x2 kw[KS];
-#pragma unroll
-            for (int i = 0; i < KS; ++i) kw[i] = *reinterpret_cast<const u32x2 *>(kp + j * 4 * D + i * 8);
             f32x4 c = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < KS; ++i) c = mma(widen8(kw[i][0], kw[i][1]), qf[i], c);
+            for (int i = 0; i < KP; ++i) {
+                if constexpr (WIDE) {
+                    const u32x4 w = now.k[j * KP + i];
+                    c = mma(widen8(w[0], w[1]), qf[2 * i], c);
+                    c = mma(widen8(w[2], w[3]), qf[2 * i + 1], c);
+                } else {
+                    const u32x2 w = now.k8[j * KP + i];
+                    c = mma(widen8(w[0], w[1]), qf[i], c);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[4 * j + i] = c[i];
         }
         const bool whole = t0 >= see_lo && t0 >= t_hi - (p.window > 0 ? p.window - 1 : INT32_MAX - 1) &&
                            t0 + kStep - 1 <= t_lo && t0 + kStep <= most;
-        const bool every = __builtin_amdgcn_ballot_w64(!in_v) == 0 && whole;  // nothing masked in this step
-        float top = -INFINITY;
+        const bool every = __builtin_amdgcn_ballot_w64(!now.in) == 0 && whole;  // nothing masked in this step
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             if constexpr (!BF) s[i] = ror_add(s[i]);
             s[i] *= ks;
-            if (!every) s[i] = (in_v && tv + i >= vis_lo && tv + i < vis_hi) ? s[i] : -INFINITY;
-            top = fmaxf(top, s[i]);
         }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float m2 = fmaxf(m, top);
-        const float ref = m2 == -INFINITY ? 0.0f : m2;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref);
-        m = m2;
+        if (!every) {
+            // codes that no row sees read as zero, and so do NaN codes, for now (nan_dims)
+            const int lo = now.in ? vis_lo - tv : 16, hi = vis_hi - tv;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
+            uint32_t keep[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) keep[i] = byte_mask(tv + 4 * i, see_lo, now.in ? see_hi : 0);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t u = now.v[d][i] & keep[i], bad = nan_bytes(u);
+                    now.v[d][i] = u & ~(bad * 0xffu);
+                    nans |= bad;
+                }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top = quads_max(top);
+        // the maximum moves only when it has grown by 2^8: weights stay within f32 and bf16 meanwhile
+        const bool grow = top > m + 8.0f || (m == -INFINITY && top > -INFINITY);
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+            const float m2 = grow ? top : m;
+            const float alpha = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m2);
+            m = m2;
+            sum *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= alpha;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
         float add = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -282,7 +376,7 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
             add += s[i];
             s[i] *= vs;
         }
-        sum = sum * alpha + add;
+        sum += add;
         u32x4 pf[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -292,47 +386,12 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
                 pf[u][i] = BF ? pair_near(a, c) : pair_cut(term_of(a, term), term_of(c, term));
             }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] *= alpha;
-        if (every) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const u32x4 v = *reinterpret_cast<const u32x4 *>(vp + (int64_t)d * 16 * P);
-                o[d] = mma(widen8(v[0], v[1]), pf[0], o[d]);
-                o[d] = mma(widen8(v[2], v[3]), pf[1], o[d]);
-            }
-        } else {
-            // Codes that no row sees read as zero.  What some rows see and others do not may be NaN, and a
-            // zero weight would not hide it: NaN codes are taken out, counted per row, and put back.
-            uint32_t keep[4], seen[4];
-            const int hi = in_v ? see_hi : 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                keep[i] = byte_mask(tv + 4 * i, see_lo, hi);
-                seen[i] = byte_mask(tv + 4 * i, vis_lo, in_v ? vis_hi : 0) & 0x01010101u;
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                u32x4 v = *reinterpret_cast<const u32x4 *>(vp + (int64_t)d * 16 * P), bad;
-                uint32_t any = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[i] &= keep[i];
-                    bad[i] = nan_bytes(v[i]);
-                    v[i] &= ~(bad[i] * 0xffu);
-                    any |= bad[i];
-                }
-                o[d] = mma(widen8(v[0], v[1]), pf[0], o[d]);
-                o[d] = mma(widen8(v[2], v[3]), pf[1], o[d]);
-                if (__builtin_amdgcn_ballot_w64(any != 0)) {
-                    // 0x38 is 1.0: counts of NaN codes that a row sees
-                    f32x4 hit = {0, 0, 0, 0};
-                    hit = mma(widen8(bad[0] * 0x38u, bad[1] * 0x38u), widen8(seen[0] * 0x38u, seen[1] * 0x38u), hit);
-                    hit = mma(widen8(bad[2] * 0x38u, bad[3] * 0x38u), widen8(seen[2] * 0x38u, seen[3] * 0x38u), hit);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[d][i] = hit[i] > 0.0f ? NAN : o[d][i];
-                }
-            }
+        for (int d = 0; d < DT; ++d) {
+            const u32x4 v = now.v[d];
+            o[d] = mma(widen8(v[0], v[1]), pf[0], o[d]);
+            o[d] = mma(widen8(v[2], v[3]), pf[1], o[d]);
         }
+        now = next;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -341,6 +400,13 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[d][i] = ror_add(o[d][i]);
+    }
+    if (__builtin_amdgcn_ballot_w64(nans != 0)) {
+        const uint64_t bits = nan_dims(p, table, head, quad, max(from, vis_lo), min(to, vis_hi));
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d][i] = (bits >> (4 * d + i)) & 1 ? NAN : o[d][i];
     }
 
     // join the 4 waves: lanes of the tile's rows put their part down, wave w takes dims w * D / 4 ..
@@ -387,11 +453,332 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
     }
 }
 
-// Joins the token splits of one query row and head.
+// ---- attention, tiles of query rows ----------------------------------------------
+//
+// Prompts: a workgroup of 4 waves owns 64 * CT query rows of one cache head (tokens x
+// the head's group of query heads) and walks the tokens 64 at a time.  The codes go to
+// LDS as they are, without passing through registers, one step ahead; every wave widens
+// them for its own CT column tiles.  f32 rows take one MFMA per term of q (3) and of
+// the weights (3) instead of a column per term, so that a weight is computed once.
+//
+// 16-byte pieces of a K row (a dim's tokens of V) are stored in an order that depends on
+// the row, so that the 8 lanes that read at a time meet different banks.
+template <int D>
+struct KvTile {
+    static constexpr int KC = D / 16;                     // pieces of a K row
+    static constexpr int K_BYTES = kStep * D, BYTES = 2 * kStep * D;
+    static constexpr int PASSES = (kStep * KC + 255) / 256;  // pieces per thread and side
+    static __device__ __forceinline__ int k_slot(int t, int c) {
+        return KC == 6 ? c : c ^ (((t & 3) | ((t >> 2) & 4)) & (KC >= 8 ? 7 : 3));
+    }
+    static __device__ __forceinline__ int v_slot(int d, int c) { return c ^ ((d >> 1) & 3); }
+};
+
+__device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i's 16 bytes to l + 16 i
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
+                                     (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
+}
+
+template <int D, bool BF, int CT>
+__global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(const KvAttend p, const KvPart part, int splits, int chunk,
+                                                          int row_tiles, int64_t rows_total) {
+    using T = KvTile<D>;
+    constexpr int PL = BF ? 1 : 3;  // terms of q and of the weights
+    constexpr int KS = D / 32, DT = D / 16, LB = D / 4, R = 64 * CT;
+    __shared__ __attribute__((aligned(16))) char lds[2][T::BYTES];
+    __shared__ int nans;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, quad = lane >> 4;
+    // heads turn fastest: with 8 of them each XCD keeps one head's codes in its L2
+    const int head = blockIdx.x % p.c.heads, rest = blockIdx.x / p.c.heads, b = blockIdx.y;
+    const int split = rest / row_tiles, tile = row_tiles - 1 - (rest - split * row_tiles);  // the longest first
+    const int group = p.q_heads / p.c.heads, P = p.c.page, lgp = 31 - __clz(P);
+    const int64_t start = p.b.starts[b];
+    const int count = (int)min((int64_t)p.b.starts[b + 1] - start, (int64_t)p.b.max_new);
+    const int row0 = tile * R, rows = count * group;
+    if (row0 >= rows) return;
+    const int len = p.b.lens[b];
+    const int here = min(R, rows - row0);
+    const int t_lo = len - count + row0 / group, t_hi = len - count + (row0 + here - 1) / group;
+    const int most = (int)min((int64_t)INT32_MAX, p.b.width * P);
+    const int see_hi = min(t_hi + 1, most);
+    const int see_lo = p.window > 0 ? max(0, t_lo - p.window + 1) : 0;
+    const int from = (see_lo & ~(kStep - 1)) + split * chunk;
+    const int to = split == splits - 1 ? see_hi : min(from + chunk, see_hi);
+    if (split > 0 && from >= see_hi) return;
+
+    u32x4 qf[CT][PL][KS];
+    int vis_lo[CT], vis_hi[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        const int my = min(row0 + (wave * CT + c) * 16 + col, rows - 1);
+        const int pos = len - count + my / group;
+        vis_lo[c] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+        vis_hi[c] = min(pos + 1, most);
+        const int64_t q0 = (start + my / group) * p.q_ld + (int64_t)(head * group + my % group) * D + quad * LB;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if constexpr (BF) {
+                struct __attribute__((packed, aligned(2))) T8 { u32x4 v; };
+                qf[c][0][s] = reinterpret_cast<const T8 *>(static_cast<const uint16_t *>(p.q) + q0 + s * 8)->v;
+            } else {
+                const float *f = static_cast<const float *>(p.q) + q0 + s * 8;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < PL; ++t) qf[c][t][s][i] = pair_cut(term_of(f[2 * i], t), term_of(f[2 * i + 1], t));
+            }
+        }
+    }
+
+    const int32_t *table = p.b.table + (int64_t)b * p.b.width;
+    const float scale = p.scale * kLog2e;
+    const int64_t page_bytes = (int64_t)P * D;
+    auto page_of = [&](int t) -> int { return t < most ? table[t >> lgp] : -1; };
+    auto safe = [&](int id) -> int64_t { return id >= 0 && id < p.c.pages ? id : 0; };
+
+    // This thread's pieces of a step: K token rows kt[], V's 16 tokens vc.
+    int kt[T::PASSES], kc[T::PASSES], vd[T::PASSES];
+    const int vslot = threadIdx.x & 3, vc = vslot ^ ((threadIdx.x >> 3) & 3);
+#pragma unroll
+    for (int i = 0; i < T::PASSES; ++i) {
+        const int at = i * 256 + threadIdx.x;
+        kt[i] = at / T::KC;
+        kc[i] = T::k_slot(kt[i], at % T::KC);
+        vd[i] = at >> 2;
+    }
+    int kid[T::PASSES], vid;
+    auto ids = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < T::PASSES; ++i) kid[i] = kt[i] < kStep ? page_of(t0 + kt[i]) : -1;
+        vid = page_of(t0 + 16 * vc);
+    };
+    auto fetch = [&](int t0, char *buf) {
+#pragma unroll
+        for (int i = 0; i < T::PASSES; ++i) {
+            if (kStep * T::KC % 256 && i == T::PASSES - 1 && wave * 64 >= kStep * T::KC % 256) break;
+            const uint8_t *k = p.c.k + (safe(kid[i]) * p.c.heads + head) * page_bytes + ((t0 + kt[i]) & (P - 1)) * D + kc[i] * 16;
+            lds_copy16(k, buf + (i * 256 + wave * 64) * 16);
+        }
+        const uint8_t *v = p.c.v + (safe(vid) * p.c.heads + head) * page_bytes + ((t0 + 16 * vc) & (P - 1));
+#pragma unroll
+        for (int i = 0; i < T::PASSES; ++i) {
+            if (kStep * T::KC % 256 && i == T::PASSES - 1 && wave * 64 >= kStep * T::KC % 256) break;
+            lds_copy16(v + vd[i] * P, buf + T::K_BYTES + (i * 256 + wave * 64) * 16);
+        }
+    };
+
+    f32x4 o[CT][DT];
+    float m[CT], sum[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        m[c] = -INFINITY;
+        sum[c] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[c][d] = f32x4{0, 0, 0, 0};
+    }
+    // where this lane's K row pieces (tokens 4 j on, piece i by its low bits) and V pieces lie
+    const int k_tok = 16 * (col >> 2) + (col & 3);
+    const int k_at = k_tok * D, k_piece = KS % 2 == 0 ? T::k_slot(k_tok, quad * (KS / 2)) * 16 : 0;
+    const int v_at = (col * 4 + T::v_slot(col, quad)) * 16;
+    int buf = 0;
+    if (threadIdx.x == 0) nans = 0;
+    if (from < to) {
+        ids(from);
+        fetch(from, lds[0]);
+        ids(from + kStep);
+    }
+    // this lane's 16 tokens: their page and its scales, a step ahead of their use
+    int own = page_of(from + 16 * quad), own_next = page_of(from + kStep + 16 * quad);
+    uint32_t ksb = p.c.ks[safe(own) * p.c.heads + head], vsb = p.c.vs[safe(own) * p.c.heads + head];
+    for (int t0 = from; t0 < to; t0 += kStep) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t0 + kStep < to) fetch(t0 + kStep, lds[buf ^ 1]);
+        ids(t0 + 2 * kStep);
+        const bool in = own >= 0 && own < p.c.pages;
+        const float ks = e8m0(ksb) * scale;
+        const uint32_t vb = vsb;
+        own = own_next;
+        own_next = page_of(t0 + 2 * kStep + 16 * quad);
+        ksb = p.c.ks[safe(own) * p.c.heads + head];
+        vsb = p.c.vs[safe(own) * p.c.heads + head];
+        const int tv = t0 + 16 * quad;
+        const bool whole = t0 >= see_lo && t0 >= t_hi - (p.window > 0 ? p.window - 1 : INT32_MAX - 1) &&
+                           t0 + kStep - 1 <= t_lo && t0 + kStep <= most;
+        const bool every = __builtin_amdgcn_ballot_w64(!in) == 0 && whole;  // nothing masked in this step
+        if (!every) {
+            // V codes that no row sees read as zero, and so do NaN codes, for now (nan_dims); every wave
+            // sees the same four pages, so the whole workgroup is here
+            const int t = t0 + 16 * vc;
+            const int id = page_of(t);
+            const int hi = id >= 0 && id < p.c.pages ? see_hi : 0;
+            uint32_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < T::PASSES; ++i) {
+                if (i * 256 + (int)threadIdx.x >= kStep * T::KC) break;
+                uint32_t *v = reinterpret_cast<uint32_t *>(lds[buf] + T::K_BYTES + (i * 256 + threadIdx.x) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t u = v[e] & byte_mask(t + 4 * e, see_lo, hi), n = nan_bytes(u);
+                    bad |= n;
+                    v[e] = u & ~(n * 0xffu);
+                }
+            }
+            if (bad) nans = 1;
+            __syncthreads();
+        }
+        const char *kb = lds[buf] + k_at, *vl = lds[buf] + T::K_BYTES + v_at;
+
+        float s[CT][16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j) __builtin_amdgcn_sched_barrier(0);
+            u32x2 w[KS];
+            if constexpr (KS % 2 == 0) {
+#pragma unroll
+                for (int i = 0; i < KS / 2; ++i) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (k_piece ^ (i * 16)));
+                    w[2 * i] = u32x2{x[0], x[1]};
+                    w[2 * i + 1] = u32x2{x[2], x[3]};
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < KS; ++i) w[i] = *reinterpret_cast<const u32x2 *>(kb + j * 4 * D + quad * LB + i * 8);
+            }
+            f32x4 acc[CT];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) acc[c] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const u32x4 a = widen8(w[i][0], w[i][1]);
+#pragma unroll
+                for (int t2 = PL - 1; t2 >= 0; --t2)
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) acc[c] = mma(a, qf[c][t2][i], acc[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[c][4 * j + i] = acc[c][i];
+        }
+
+        __builtin_amdgcn_sched_barrier(0);
+        // V's scale enters the weight through the exponent, but where that could leave the exponent's range
+        const bool fold = vb >= 67 && vb <= 187;
+        const float shift = fold ? (float)((int)vb - 127) : 0.0f;
+        const float unfold = fold ? e8m0(254 - vb) : 1.0f;
+        const bool plain = __builtin_amdgcn_ballot_w64(!fold) != 0;
+        u32x4 pf[CT][PL][2];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            if (!every) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[c][i] = (in && tv + i >= vis_lo[c] && tv + i < vis_hi[c]) ? s[c][i] : -INFINITY;
+            }
+            float top = s[c][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[c][i]);
+            top = quads_max(top * ks);
+            // the maximum moves only when it has grown by 2^8: weights stay within f32 and bf16 meanwhile
+            const bool grow = top > m[c] + 8.0f || (m[c] == -INFINITY && top > -INFINITY);
+            if (__builtin_amdgcn_ballot_w64(grow)) {
+                const float m2 = grow ? top : m[c];
+                const float alpha = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[c] - m2);
+                m[c] = m2;
+                sum[c] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[c][d] *= alpha;
+            }
+            const float off = shift - (m[c] == -INFINITY ? 0.0f : m[c]);
+            float add = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i], ks, off));
+                add += s[c][i];
+            }
+            sum[c] = fmaf(add, unfold, sum[c]);
+            if (plain) {
+                const float vs = fold ? 1.0f : e8m0(vb);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[c][i] *= vs;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = s[c][8 * u + 2 * i], y = s[c][8 * u + 2 * i + 1];
+                    if constexpr (BF) {
+                        pf[c][0][u][i] = pair_near(x, y);
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < PL; ++t) pf[c][t][u][i] = pair_cut(term_of(x, t), term_of(y, t));
+                    }
+                }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(vl + d * 1024);
+            const u32x4 a0 = widen8(v[0], v[1]), a1 = widen8(v[2], v[3]);
+#pragma unroll
+            for (int t = PL - 1; t >= 0; --t)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    o[c][d] = mma(a0, pf[c][t][0], o[c][d]);
+                    o[c][d] = mma(a1, pf[c][t][1], o[c][d]);
+                }
+        }
+        buf ^= 1;
+    }
+
+    __syncthreads();
+    if (nans) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const uint64_t bits = nan_dims(p, table, head, quad, max(from, vis_lo[c]), min(to, vis_hi[c]));
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[c][d][i] = (bits >> (4 * d + i)) & 1 ? NAN : o[c][d][i];
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        sum[c] += __shfl_xor(sum[c], 16);
+        sum[c] += __shfl_xor(sum[c], 32);
+        const int r = row0 + (wave * CT + c) * 16 + col;
+        if (r >= rows) continue;
+        const int h = head * group + r % group;
+        if (splits == 1) {
+            const float inv = sum[c] == 0.0f ? 0.0f : 1.0f / sum[c];  // nothing seen: zero
+            const int64_t at = (start + r / group) * p.out_ld + (int64_t)h * D + quad * 4;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (BF) static_cast<__bf16 *>(p.out)[at + d * 16 + i] = (__bf16)(o[c][d][i] * inv);
+                    else static_cast<float *>(p.out)[at + d * 16 + i] = o[c][d][i] * inv;
+                }
+        } else {
+            const int64_t at = ((int64_t)split * rows_total + (int64_t)b * p.b.max_new + r / group) * p.q_heads + h;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(part.o + at * D + d * 16 + quad * 4) = o[c][d];
+            if (quad == 0) {
+                part.ml[at * 2] = m[c];
+                part.ml[at * 2 + 1] = sum[c];
+            }
+        }
+    }
+}
+
+// Joins the token splits of one query row and head: wave w takes every fourth split, a lane dims lane, lane + 64, ..
 template <bool BF>
 __global__ __launch_bounds__(256) void kv_join_kernel(const KvAttend p, const KvPart part, int splits, int chunk,
                                                       int rows_per_tile, int64_t rows_total) {
     const int b = blockIdx.z, h = blockIdx.y, D = p.c.dim;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int group = p.q_heads / p.c.heads;
     const int64_t start = p.b.starts[b];
     const int count = (int)min((int64_t)p.b.starts[b + 1] - start, (int64_t)p.b.max_new);
@@ -407,33 +794,62 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvAttend p, const Kv
     const int used = max(1, min(splits, (span + chunk - 1) / chunk));
     const int64_t at = ((int64_t)b * p.b.max_new + i) * p.q_heads + h, step = rows_total * p.q_heads;
     float top = -INFINITY;
-    for (int s = 0; s < used; ++s) top = fmaxf(top, part.ml[(at + s * step) * 2]);
+    for (int s = lane; s < used; s += 64) top = fmaxf(top, part.ml[(at + s * step) * 2]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float ref = top == -INFINITY ? 0.0f : top;
-    for (int d = threadIdx.x; d < D; d += 256) {
-        float val = 0.0f, tot = 0.0f;
-        for (int s = 0; s < used; ++s) {
-            const float f = __builtin_amdgcn_exp2f(part.ml[(at + s * step) * 2] - ref);
-            tot += f * part.ml[(at + s * step) * 2 + 1];
-            val += f * part.o[(at + s * step) * D + d];
-        }
-        const float o = tot == 0.0f ? 0.0f : val / tot;
-        const int64_t to = (start + i) * p.out_ld + (int64_t)h * D + d;
-        if constexpr (BF) static_cast<__bf16 *>(p.out)[to] = (__bf16)o;
-        else static_cast<float *>(p.out)[to] = o;
+    float val[4] = {0, 0, 0, 0}, tot = 0.0f;
+#pragma unroll 4
+    for (int s = wave; s < used; s += 4) {
+        const float f = __builtin_amdgcn_exp2f(part.ml[(at + s * step) * 2] - ref);
+        tot += f * part.ml[(at + s * step) * 2 + 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (lane + 64 * j < D) val[j] += f * part.o[(at + s * step) * D + lane + 64 * j];
     }
+    __shared__ float vals[4][256], tots[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vals[wave][lane + 64 * j] = val[j];
+    if (lane == 0) tots[wave] = tot;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    tot = (tots[0] + tots[1]) + (tots[2] + tots[3]);
+    const float sum = (vals[0][d] + vals[1][d]) + (vals[2][d] + vals[3][d]);
+    const float o = tot == 0.0f ? 0.0f : sum / tot;
+    const int64_t to = (start + i) * p.out_ld + (int64_t)h * D + d;
+    if constexpr (BF) static_cast<__bf16 *>(p.out)[to] = (__bf16)o;
+    else static_cast<float *>(p.out)[to] = o;
+}
+
+// Column tiles per wave: as many as 256 registers hold.
+template <int D, bool BF>
+constexpr int kTiles = BF && D <= 128 ? 2 : 1;
+
+// Query rows of one head that a workgroup owns.
+int tile_rows(const KvAttend &p, int kind) {
+    if (kind == 0) return p.bf16 ? 16 : 4;
+    return 64 * (p.bf16 && p.c.dim <= 128 ? 2 : 1);
 }
 
 template <bool BF>
-hipError_t attend_rows(const KvAttend &p, const KvPlan &pl, void *workspace, hipStream_t stream) {
-    const int group = p.q_heads / p.c.heads, R = BF ? 16 : 4;
+hipError_t attend(const KvAttend &p, const KvPlan &pl, void *workspace, hipStream_t stream) {
+    const int group = p.q_heads / p.c.heads, R = tile_rows(p, pl.kind);
     const int row_tiles = (p.b.max_new * group + R - 1) / R;
     const int64_t rows_total = (int64_t)p.b.batch * p.b.max_new;
     KvPart part{};
     part.o = static_cast<float *>(workspace);
     part.ml = part.o + (size_t)pl.splits * rows_total * p.q_heads * p.c.dim;
-    const dim3 grid((unsigned)(pl.splits * row_tiles), (unsigned)p.c.heads, (unsigned)p.b.batch);
-#define DMC_DIM(N) \
-    case N: kv_rows_kernel<N, BF><<<grid, dim3(256), 0, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total); break;
+    const dim3 rows_grid((unsigned)(pl.splits * row_tiles), (unsigned)p.c.heads, (unsigned)p.b.batch);
+    const dim3 tiles_grid((unsigned)(pl.splits * row_tiles * p.c.heads), (unsigned)p.b.batch);
+#define DMC_DIM(N)                                                                                                        \
+    case N:                                                                                                               \
+        if (pl.kind == 0)                                                                                                 \
+            kv_rows_kernel<N, BF><<<rows_grid, dim3(256), 0, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total); \
+        else                                                                                                              \
+            kv_tiles_kernel<N, BF, kTiles<N, BF>>                                                                         \
+                <<<tiles_grid, dim3(256), 0, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total);              \
+        break;
     switch (p.c.dim) {
         DMC_DIM(64)
         DMC_DIM(96)
@@ -464,14 +880,18 @@ hipError_t launch_kv_append(const KvAppend &p, hipStream_t stream) {
 
 KvPlan plan_kv(const KvAttend &p, int num_cus) {
     KvPlan pl{};
-    const int group = p.q_heads / p.c.heads, R = p.bf16 ? 16 : 4;
+    const int group = p.q_heads / p.c.heads;
+    pl.kind = p.b.max_new * group > 16 ? 1 : 0;
+    const int R = tile_rows(p, pl.kind);
     const int64_t tiles = (int64_t)((p.b.max_new * group + R - 1) / R) * p.c.heads * p.b.batch;
+    const int64_t unit = pl.kind ? kStep : 4 * kStep;  // tokens of a workgroup's step
     int64_t span = p.b.max_len;
     if (p.window > 0) span = std::min<int64_t>(span, p.window + R + kStep);
-    const int64_t units = std::max<int64_t>(1, (span + 4 * kStep - 1) / (4 * kStep));
-    const int64_t want = std::max<int64_t>(1, 4 * num_cus / std::max<int64_t>(1, tiles));
-    const int64_t per = (units + want - 1) / want;  // steps of 256 tokens per workgroup
-    pl.chunk = (int)(per * 4 * kStep);
+    const int64_t units = std::max<int64_t>(1, (span + unit - 1) / unit);
+    const int64_t want = std::max<int64_t>(1, (pl.kind ? 2 : 8) * num_cus / std::max<int64_t>(1, tiles));
+    // steps per workgroup: a split of few costs more in its partial results than it saves
+    const int64_t per = std::max<int64_t>((units + want - 1) / want, pl.kind ? 8 : 4);
+    pl.chunk = (int)(per * unit);
     pl.splits = (int)((units + per - 1) / per);
     if (pl.splits > 1)
         pl.workspace_bytes = (size_t)pl.splits * p.b.batch * p.b.max_new * p.q_heads * (p.c.dim + 2) * 4;
@@ -479,7 +899,7 @@ KvPlan plan_kv(const KvAttend &p, int num_cus) {
 }
 
 hipError_t launch_kv_attend(const KvAttend &p, const KvPlan &pl, void *workspace, hipStream_t stream) {
-    return p.bf16 ? attend_rows<true>(p, pl, workspace, stream) : attend_rows<false>(p, pl, workspace, stream);
+    return p.bf16 ? attend<true>(p, pl, workspace, stream) : attend<false>(p, pl, workspace, stream);
 }
 
 }  // namespace dmc
