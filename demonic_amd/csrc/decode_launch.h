@@ -43,7 +43,9 @@ struct MxProblem {
 struct MxPlan {
     int kind;        // 0: rows (f32 x, few activation rows), 1: tiles
     int tiles;       // rows: 16-row weight tiles per workgroup
-    int64_t grid_x, grid_y;
+    int shape;       // tiles: which tile shape
+    int slices, per; // tiles: slices of k, groups of 128 in each
+    int64_t grid_x;
     size_t workspace_bytes;
 };
 MxPlan plan_mx(const MxProblem &p, int num_cus);

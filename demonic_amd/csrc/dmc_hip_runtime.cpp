@@ -1466,6 +1466,7 @@ int kv_args(const dmc_hip_kv8 *cache, const dmc_hip_kv8_batch *batch, int64_t dt
         return fail(DMC_HIP_EINVAL, "null cache pointer");
     if (cache->k_dev % 16 || cache->v_dev % 16) return fail(DMC_HIP_EINVAL, "cache pages must be 16-byte aligned");
     if (batch->batch > 0 && batch->max_new > 0) {
+        if (batch->width < 1) return fail(DMC_HIP_EINVAL, "a page table of no width");
         if (!batch->table_dev || !batch->lens_dev || !batch->starts_dev) return fail(DMC_HIP_EINVAL, "null batch pointer");
         if (batch->table_dev % 4 || batch->lens_dev % 4 || batch->starts_dev % 4)
             return fail(DMC_HIP_EINVAL, "misaligned batch pointer");

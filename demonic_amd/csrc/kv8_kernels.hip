@@ -247,7 +247,10 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
     const int32_t *table = p.b.table + (int64_t)b * p.b.width;
     const float scale = p.scale * kLog2e;
     const int64_t page_bytes = (int64_t)P * D;
-    auto page_of = [&](int t) -> int { return t < most ? table[t >> lgp] : -1; };
+    auto page_of = [&](int t) -> int {  // no branch: past the table, its last entry is read and not taken
+        const int id = table[min(t, most - 1) >> lgp];
+        return t < most ? id : -1;
+    };
     auto safe = [&](int id) -> int64_t { return id >= 0 && id < p.c.pages ? id : 0; };
     struct Codes {
         u32x4 v[DT];
@@ -534,7 +537,10 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
     const int32_t *table = p.b.table + (int64_t)b * p.b.width;
     const float scale = p.scale * kLog2e;
     const int64_t page_bytes = (int64_t)P * D;
-    auto page_of = [&](int t) -> int { return t < most ? table[t >> lgp] : -1; };
+    auto page_of = [&](int t) -> int {  // no branch: past the table, its last entry is read and not taken
+        const int id = table[min(t, most - 1) >> lgp];
+        return t < most ? id : -1;
+    };
     auto safe = [&](int id) -> int64_t { return id >= 0 && id < p.c.pages ? id : 0; };
 
     // This thread's pieces of a step: K token rows kt[], V's 16 tokens vc.

@@ -319,24 +319,21 @@ size_t rows_lds(int tiles, int m) {
 // 2^(e - 5 p), and the five products add up to x's at 24 bits of the block's
 // largest value, as a sum in f32 of such products has them.
 //
-// The planes of x: for each group of 128 k, each 16 activation rows and each digit
-// 64 lanes x 24 bytes, and per group and 16 rows 64 x 8 bytes of scales (the
-// digits' bytes, the first first).  A row that holds an inf or a NaN is marked and
-// its outputs are summed product by product instead.
+// x's digits: for each group of 128 k and each 16 activation rows 8 KB, digit by digit 64 lanes x 16 bytes and
+// 64 x 8 bytes, and after the digits 64 x 8 bytes of scales (the digits' bytes, the first first).  A block that
+// holds an inf or a NaN has scale 255, so that its row's outputs come out NaN; an output that does is summed
+// again, product by product, which gives the formula's class.
 constexpr int kDigits = 5;
-constexpr int kPlaneBytes = 64 * 24;
+constexpr int kUnit = 8192, kUnitScales = kDigits * 1536;
 
-size_t planes_bytes(int64_t m, int64_t k) { return (size_t)(mx_groups(k) * ((m + 15) / 16)) * (kDigits * kPlaneBytes + 512); }
+size_t digits_bytes(int64_t m, int64_t k) { return (size_t)(mx_groups(k) * ((m + 15) / 16)) * kUnit; }
 
-__global__ __launch_bounds__(256) void mx_split_kernel(const float *__restrict__ x, char *__restrict__ planes,
-                                                       u32x2 *__restrict__ scales, uint32_t *__restrict__ marks,
-                                                       int m, int k, int groups, int rtiles) {
+__global__ __launch_bounds__(256) void mx_split_kernel(const float *__restrict__ x, char *__restrict__ digits, int m,
+                                                       int k, int rtiles) {
     // 4 lanes per block of 32: lane j has values 8 j .. 8 j + 7
-    const int j = threadIdx.x & 3;
-    const int64_t b = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 2;  // (group, row tile, lane)
-    const int64_t unit = b >> 6;
-    if (unit >= (int64_t)groups * rtiles) return;
-    const int lane = (int)(b & 63), g = (int)(unit / rtiles), rt = (int)(unit - (int64_t)g * rtiles);
+    const int j = threadIdx.x & 3, lane = threadIdx.x >> 2;
+    const int64_t unit = blockIdx.x;
+    const int g = (int)(unit / rtiles), rt = (int)(unit - (int64_t)g * rtiles);
     const int row = rt * 16 + (lane & 15), at = g * 128 + (lane >> 4) * 32 + j * 8;
     MxIn<false> v;
     v.load(x, (int64_t)min(row, m - 1) * k + at, row < m ? max(0, k - at) : 0);
@@ -344,14 +341,13 @@ __global__ __launch_bounds__(256) void mx_split_kernel(const float *__restrict__
     const bool bad = amax >= 0x7f800000u;
     // the first digit's scale byte: amax in [2, 4) of it; 20 at least, so that the last digit's is one
     const int base = max((int)(amax >> 23) - 1, 20);
-    if (bad && j == 0) atomicOr(&marks[row >> 5], 1u << (row & 31));
     int num[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float f = ldexpf(__uint_as_float(v.u[i]), 149 - base);
         num[i] = bad ? 0 : (int)rintf(f);
     }
-    char *o = planes + unit * (kDigits * kPlaneBytes) + lane * 24 + j * 6;
+    char *o = digits + unit * kUnit;
 #pragma unroll
     for (int p = kDigits - 1; p >= 0; --p) {
         uint64_t bits = 0;
@@ -363,18 +359,21 @@ __global__ __launch_bounds__(256) void mx_split_kernel(const float *__restrict__
             // e2m3 of a / 4: eighths below 2, quarters from there
             bits |= (uint64_t)((a + min(a, 8u)) | (d < 0 ? 32u : 0u)) << (6 * i);
         }
-        uint16_t *w = reinterpret_cast<uint16_t *>(o + p * kPlaneBytes);
-        w[0] = (uint16_t)bits;
-        w[1] = (uint16_t)(bits >> 16);
-        w[2] = (uint16_t)(bits >> 32);
+#pragma unroll
+        for (int h = 0; h < 3; ++h) {
+            const int byte = j * 6 + 2 * h;
+            char *w = o + p * 1536 + (byte < 16 ? lane * 16 + byte : 1024 + lane * 8 + byte - 16);
+            *reinterpret_cast<uint16_t *>(w) = (uint16_t)(bits >> (16 * h));
+        }
     }
     if (j == 0) {
         const uint32_t s = (uint32_t)base;
-        scales[unit * 64 + lane] = u32x2{s | (s - 5) << 8 | (s - 10) << 16 | (s - 15) << 24, s - 20};
+        *reinterpret_cast<u32x2 *>(o + kUnitScales + lane * 8) =
+            bad ? u32x2{~0u, ~0u} : u32x2{s | (s - 5) << 8 | (s - 10) << 16 | (s - 15) << 24, s - 20};
     }
 }
 
-// One output of a marked row, product by product.
+// One output of f32 x, product by product.
 __device__ float mx_plain_dot(const float *x, const uint8_t *wq, const uint8_t *ws, int k) {
     float sum = 0.0f;
     for (int i = 0; i < k; ++i) {
@@ -386,103 +385,198 @@ __device__ float mx_plain_dot(const float *x, const uint8_t *wq, const uint8_t *
 }
 
 struct MxTileArgs {
-    const float *x;
+    const float *x;            // f32 x (its digits in xq), or null
     const uint8_t *xq, *xs, *wq, *ws;
-    const char *planes;
-    const u32x2 *scales;
-    const uint32_t *marks;
-    float *y;
+    float *y;                  // or the slices' partial sums [slice][m][n]
     int m, k, n, groups, rtiles;
+    int ntn, ntm;              // tiles along n and m
+    int slices, per;           // slices of k, groups of each
 };
 
-template <int PL, int RT, int CT>
-__global__ __launch_bounds__(256) void mx_tile_kernel(const MxTileArgs p) {
+__device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i's 16 bytes to l + 16 i
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
+                                     (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
+}
+__device__ __forceinline__ void lds_copy4(const void *g, char *l) {  // lane i's 4 bytes to l + 4 i
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
+                                     (__attribute__((address_space(3))) uint32_t *)l, 4, 0, 0);
+}
+
+// Tiles of TN weight rows x TM activation rows; WN x WM waves of RT x CT MFMA tiles.  Both sides go to LDS without
+// passing through registers, SK groups of 128 k per stage, three stages deep, in the order that a lane reads its
+// operands in (16 rows x 4 blocks: lane 16 q + r's 16 bytes at 16 (16 q + r)), so that reads meet no bank twice.
+template <int PL, int RT, int CT, int WN, int WM, int SK>
+struct MxTile {
+    static constexpr int kWaves = WN * WM, TN = WN * RT * 16, TM = WM * CT * 16;
+    static constexpr int kWq = TN * 64, kWs = (TN + 63) / 64 * 256;
+    static constexpr int kXq = PL == 1 ? TM * 64 : TM / 16 * kUnit, kXs = PL == 1 ? (TM + 63) / 64 * 256 : 0;
+    static constexpr int kGroup = kWq + kXq + kWs + kXs;  // LDS bytes of a group of k
+    static constexpr int kStage = SK * kGroup;
+    static constexpr int kBig = (kWq + kXq) / 1024, kSmall = (kWs + kXs) / 256;  // copies of a group
+    static constexpr int kBigEach = (kBig * SK + kWaves - 1) / kWaves, kSmallEach = (kSmall * SK + kWaves - 1) / kWaves;
+    static constexpr int kCopies = kBigEach + kSmallEach;  // of a wave per stage
+    static constexpr int kDepth = 3;
+    static_assert(kDepth * kStage <= 160 * 1024 && kCopies < 32, "");
+};
+
+template <int PL, int RT, int CT, int WN, int WM, int SK>
+__global__ __launch_bounds__(64 * WN * WM) void mx_tile_kernel(const MxTileArgs p) {
+    using T = MxTile<PL, RT, CT, WN, WM, SK>;
+    extern __shared__ char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, quad = lane >> 4;
-    const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * RT * 16;
-    const int m0 = blockIdx.y * CT * 16;
-    if (n0 >= p.n) return;
+    const int wn = wave % WN, wm = wave / WN;
+    // consecutive workgroups go to the 8 XCDs in turn: give each XCD neighbouring tiles, 4 along n at a time
+    const int tiles = p.ntn * p.ntm, each = (tiles + 7) / 8;
+    const int id = ((int)blockIdx.x & 7) * each + ((int)blockIdx.x >> 3);
+    if (((int)blockIdx.x >> 3) >= each || id >= tiles) return;
+    const int band = id / (4 * p.ntm), in = id - band * 4 * p.ntm, wide = min(4, p.ntn - 4 * band);
+    const int tn = band * 4 + in % wide, tm = in / wide;
+    const int slice = blockIdx.y;
+    const int g0 = slice * p.per, g1 = min(p.groups, g0 + p.per);
+    const int64_t n0 = (int64_t)tn * T::TN;
+    const int m0 = tm * T::TM;
     const int64_t qrow = (int64_t)p.groups * 64, srow = (int64_t)p.groups * 4;
-    const uint8_t *wq[RT], *ws[RT], *xq[CT], *xs[CT];
+
+    // this wave's copies of a stage (past the last one: the last one again)
+    const uint8_t *big[T::kBigEach], *small_[T::kSmallEach];
+    int big_lds[T::kBigEach], small_lds[T::kSmallEach], big_g[T::kBigEach], small_g[T::kSmallEach];
+    bool big_x[T::kBigEach];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const int64_t row = min(n0 + i * 16 + r, (int64_t)p.n - 1);
-        wq[i] = p.wq + row * qrow + quad * 16;
-        ws[i] = p.ws + row * srow + quad;
+    for (int i = 0; i < T::kBigEach; ++i) {
+        const int c = min(wave + i * T::kWaves, T::kBig * SK - 1), half = c / T::kBig, at = c - half * T::kBig;
+        big_g[i] = half;
+        big_lds[i] = half * T::kGroup + at * 1024;
+        big_x[i] = at >= T::kWq / 1024;
+        if (!big_x[i]) {
+            const int64_t row = min(n0 + at * 16 + r, (int64_t)p.n - 1);
+            big[i] = p.wq + row * qrow + quad * 16;
+        } else if (PL == 1) {
+            const int64_t row = min(m0 + (at - T::kWq / 1024) * 16 + r, p.m - 1);
+            big[i] = p.xq + row * qrow + quad * 16;
+        } else {
+            const int xt = at - T::kWq / 1024, tile = min((m0 >> 4) + (xt >> 3), p.rtiles - 1);
+            big[i] = p.xq + (int64_t)tile * kUnit + (xt & 7) * 1024 + lane * 16;
+        }
     }
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
-        const int64_t row = min(m0 + i * 16 + r, p.m - 1);
-        xq[i] = PL == 1 ? p.xq + row * qrow + quad * 16 : nullptr;
-        xs[i] = PL == 1 ? p.xs + row * srow + quad : nullptr;
+    for (int i = 0; i < T::kSmallEach; ++i) {
+        const int c = min(wave + i * T::kWaves, T::kSmall * SK - 1), half = c / T::kSmall, at = c - half * T::kSmall;
+        small_g[i] = half;
+        small_lds[i] = half * T::kGroup + T::kWq + T::kXq + at * 256;
+        if (at < T::kWs / 256) small_[i] = p.ws + min(n0 + at * 64 + lane, (int64_t)p.n - 1) * srow;
+        else small_[i] = p.xs + (int64_t)min(m0 + (at - T::kWs / 256) * 64 + lane, p.m - 1) * srow;
     }
+    auto copy = [&](int g, char *to) {  // groups past the slice's end: its last one
+#pragma unroll
+        for (int i = 0; i < T::kBigEach; ++i) {
+            const int64_t at = min(g + big_g[i], g1 - 1);
+            lds_copy16(big[i] + (PL > 1 && big_x[i] ? at * p.rtiles * kUnit : at * 64), to + big_lds[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < T::kSmallEach; ++i) lds_copy4(small_[i] + (int64_t)min(g + small_g[i], g1 - 1) * 4, to + small_lds[i]);
+    };
+
     f32x4 acc[RT][CT];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < CT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    for (int g = 0; g < p.groups; ++g) {
-        i32x8 a[RT];
-        int as[RT];
+    copy(g0, lds);
+    copy(g0 + SK, lds + T::kStage);
+    int stage = 0;
+    for (int g = g0; g < g1; g += SK) {
+        // this stage has arrived (the next may be in flight) and the last one's reads are done
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kCopies) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int into = stage + 2 >= T::kDepth ? stage + 2 - T::kDepth : stage + 2;
+        copy(g + 2 * SK, lds + into * T::kStage);
+        const char *base = lds + stage * T::kStage;
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const u32x4 t = *reinterpret_cast<const u32x4 *>(wq[i] + (int64_t)g * 64);
-            a[i] = i32x8{(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
-            as[i] = ws[i][(int64_t)g * 4];
-        }
+        for (int h = 0; h < SK; ++h) {
+            if (h && g + h >= g1) break;
+            const char *gb = base + h * T::kGroup;
+            i32x8 a[RT];
+            int as[RT];
 #pragma unroll
-        for (int j = 0; j < CT; ++j) {
-            if constexpr (PL == 1) {
-                const u32x4 t = *reinterpret_cast<const u32x4 *>(xq[j] + (int64_t)g * 64);
-                const i32x8 b = {(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
-                const int bs = xs[j][(int64_t)g * 4];
+            for (int i = 0; i < RT; ++i) {
+                const u32x4 t = *reinterpret_cast<const u32x4 *>(gb + ((wn * RT + i) * 64 + lane) * 16);
+                a[i] = i32x8{(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
+                as[i] = *reinterpret_cast<const uint8_t *>(gb + T::kWq + T::kXq + ((wn * RT + i) * 16 + r) * 4 + quad);
+            }
 #pragma unroll
-                for (int i = 0; i < RT; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 4, 0, as[i], 0, bs);
-            } else {
-                const int64_t unit = (int64_t)g * p.rtiles + min((m0 >> 4) + j, p.rtiles - 1);
-                const u32x2 sc = p.scales[unit * 64 + lane];
-                const char *pb = p.planes + unit * (PL * kPlaneBytes) + lane * 24;
-#define DMC_DIGIT(P, SEL, WORD)                                                                                     \
-    {                                                                                                               \
-        const u32x2 *t = reinterpret_cast<const u32x2 *>(pb + P * kPlaneBytes);                                     \
-        const u32x2 t0 = t[0], t1 = t[1], t2 = t[2];                                                                \
-        const i32x8 b = {(int)t0[0], (int)t0[1], (int)t1[0], (int)t1[1], (int)t2[0], (int)t2[1], 0, 0};             \
-        _Pragma("unroll") for (int i = 0; i < RT; ++i) acc[i][j] =                                                  \
+            for (int j = 0; j < CT; ++j) {
+                if constexpr (PL == 1) {
+                    const u32x4 t = *reinterpret_cast<const u32x4 *>(gb + T::kWq + ((wm * CT + j) * 64 + lane) * 16);
+                    const i32x8 b = {(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
+                    const int bs = *reinterpret_cast<const uint8_t *>(gb + T::kWq + T::kXq + T::kWs + ((wm * CT + j) * 16 + r) * 4 + quad);
+#pragma unroll
+                    for (int i = 0; i < RT; ++i)
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 4, 0, as[i], 0, bs);
+                } else {
+                    const char *xb = gb + T::kWq + (wm * CT + j) * kUnit;
+                    const u32x2 sc = *reinterpret_cast<const u32x2 *>(xb + kUnitScales + lane * 8);
+#define DMC_DIGIT(P, SEL, WORD)                                                                                       \
+    {                                                                                                                 \
+        const u32x4 t0 = *reinterpret_cast<const u32x4 *>(xb + P * 1536 + lane * 16);                                 \
+        const u32x2 t1 = *reinterpret_cast<const u32x2 *>(xb + P * 1536 + 1024 + lane * 8);                           \
+        const i32x8 b = {(int)t0[0], (int)t0[1], (int)t0[2], (int)t0[3], (int)t1[0], (int)t1[1], 0, 0};               \
+        _Pragma("unroll") for (int i = 0; i < RT; ++i) acc[i][j] =                                                    \
             __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 2, 0, as[i], SEL, (int)sc[WORD]); \
     }
-                DMC_DIGIT(4, 0, 1)
-                DMC_DIGIT(3, 3, 0)
-                DMC_DIGIT(2, 2, 0)
-                DMC_DIGIT(1, 1, 0)
-                DMC_DIGIT(0, 0, 0)
+                    DMC_DIGIT(4, 0, 1)
+                    DMC_DIGIT(3, 3, 0)
+                    DMC_DIGIT(2, 2, 0)
+                    DMC_DIGIT(1, 1, 0)
+                    DMC_DIGIT(0, 0, 0)
 #undef DMC_DIGIT
+                }
             }
         }
+        stage = stage + 1 == T::kDepth ? 0 : stage + 1;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives its workgroup's LDS
+    float *y = p.y + (int64_t)slice * p.m * p.n;
 #pragma unroll
     for (int j = 0; j < CT; ++j) {
-        const int col = m0 + j * 16 + r;
+        const int col = m0 + (wm * CT + j) * 16 + r;
         if (col >= p.m) continue;
-        const bool marked = PL > 1 && (p.marks[col >> 5] >> (col & 31) & 1u);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            const int64_t row = n0 + i * 16 + quad * 4;
+            const int64_t row = n0 + (wn * RT + i) * 16 + quad * 4;
+            f32x4 v = acc[i][j];
+            if (PL > 1 && p.slices == 1) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (row + e >= p.n) continue;
-                float v = acc[i][j][e];
-                if (marked)
-                    v = mx_plain_dot(p.x + (int64_t)col * p.k, p.wq + (row + e) * qrow, p.ws + (row + e) * srow, p.k);
-                p.y[(int64_t)col * p.n + row + e] = v;
+                for (int e = 0; e < 4; ++e)
+                    if (__builtin_isnan(v[e]) && row + e < p.n)
+                        v[e] = mx_plain_dot(p.x + (int64_t)col * p.k, p.wq + (row + e) * qrow, p.ws + (row + e) * srow, p.k);
+            }
+            float *o = y + (int64_t)col * p.n + row;
+            struct __attribute__((packed, aligned(4))) F4 { f32x4 v; };
+            if (row + 4 <= p.n) {
+                reinterpret_cast<F4 *>(o)->v = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (row + e < p.n) o[e] = v[e];
             }
         }
     }
 }
 
-__global__ void mx_clear_kernel(uint32_t *p, int n) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = 0;
+// y = the slices' partial sums, in slice order; an f32 row's NaN as in the tile kernel.
+__global__ __launch_bounds__(256) void mx_sum_kernel(const MxTileArgs p, float *__restrict__ y) {
+    const int64_t total = (int64_t)p.m * p.n;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        float s = p.y[i];
+        for (int k = 1; k < p.slices; ++k) s += p.y[k * total + i];
+        if (p.x && __builtin_isnan(s)) {
+            const int64_t col = i / p.n, row = i - col * p.n;
+            s = mx_plain_dot(p.x + col * p.k, p.wq + row * p.groups * 64, p.ws + row * p.groups * 4, p.k);
+        }
+        y[i] = s;
+    }
 }
 
 __global__ void mx_zero_kernel(float *y, int64_t n) {
@@ -509,6 +603,44 @@ hipError_t launch_mx_dequantize(const MxCast &p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// The tile shapes, by number: template arguments, and a launch of each.
+#define DMC_MX_SHAPES(X)                                            \
+    X(0, 1, 8, 4, 2, 2, 2) /* 256 x 128 */                          \
+    X(1, 1, 2, 4, 4, 1, 2) /* 128 x 64 */                           \
+    X(2, 1, 1, 1, 4, 1, 2) /* 64 x 16 */                            \
+    X(3, kDigits, 8, 2, 2, 2, 1) /* 256 x 64 */                     \
+    X(4, kDigits, 2, 2, 4, 1, 1) /* 128 x 32 */                     \
+    X(5, kDigits, 1, 1, 4, 1, 1) /* 64 x 16 */                      \
+    X(6, kDigits, 4, 1, 4, 1, 1) /* 256 x 16 */
+
+namespace {
+struct Shape { int tn, tm; };
+constexpr Shape kShapes[] = {
+#define X(ID, PL, RT, CT, WN, WM, SK) {WN * RT * 16, WM * CT * 16},
+    DMC_MX_SHAPES(X)
+#undef X
+};
+
+hipError_t launch_shape(int shape, const MxTileArgs &a, hipStream_t stream) {
+    const dim3 grid((unsigned)((a.ntn * a.ntm + 7) / 8 * 8), (unsigned)a.slices);
+    switch (shape) {
+#define X(ID, PL, RT, CT, WN, WM, SK)                                                                                   \
+    case ID: {                                                                                                        \
+        auto f = mx_tile_kernel<PL, RT, CT, WN, WM, SK>;                                                               \
+        constexpr int lds = MxTile<PL, RT, CT, WN, WM, SK>::kDepth * MxTile<PL, RT, CT, WN, WM, SK>::kStage;           \
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(f),                                    \
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, lds);                     \
+        if (e != hipSuccess) return e;                                                                                 \
+        f<<<grid, dim3(64 * WN * WM), lds, stream>>>(a);                                                               \
+        return hipGetLastError();                                                                                      \
+    }
+        DMC_MX_SHAPES(X)
+#undef X
+    }
+    return hipErrorInvalidValue;
+}
+}  // namespace
+
 MxPlan plan_mx(const MxProblem &p, int num_cus) {
     MxPlan pl{};
     if (p.k == 0) return pl;
@@ -517,13 +649,24 @@ MxPlan plan_mx(const MxProblem &p, int num_cus) {
         const int64_t tiles = (p.n + 15) / 16;
         pl.tiles = tiles >= 8 * 4 * (int64_t)num_cus ? 8 : tiles >= 2 * 4 * (int64_t)num_cus ? 2 : 1;
         pl.grid_x = (tiles + pl.tiles - 1) / pl.tiles;
-        pl.grid_y = 1;
-    } else {
-        pl.kind = 1;
-        pl.grid_x = div_up(p.n, 4 * 2 * 16);
-        pl.grid_y = div_up(p.m, 2 * 16);
-        if (p.x) pl.workspace_bytes = planes_bytes(p.m, p.k) + (size_t)((p.m + 31) / 32) * 4;
+        return pl;
     }
+    pl.kind = 1;
+    const int64_t groups = mx_groups(p.k);
+    if (!p.x) pl.shape = p.m > 64 ? 0 : p.m > 16 ? 1 : 2;
+    else pl.shape = p.m > 32 ? 3 : p.m > 16 ? 4 : p.n >= 256 * (int64_t)num_cus ? 6 : 5;
+    const Shape s = kShapes[pl.shape];
+    pl.grid_x = (int64_t)div_up(p.n, s.tn) * div_up(p.m, s.tm);
+    // k is cut where the tiles alone leave CUs without one
+    pl.slices = 1;
+    if (pl.grid_x < num_cus) {
+        const int64_t most = std::max<int64_t>(1, groups / 8);
+        pl.slices = (int)std::min<int64_t>(most, num_cus / pl.grid_x);
+    }
+    pl.per = (int)((groups + pl.slices - 1) / pl.slices);
+    pl.slices = (int)((groups + pl.per - 1) / pl.per);
+    pl.workspace_bytes = p.x ? digits_bytes(p.m, p.k) : 0;
+    if (pl.slices > 1) pl.workspace_bytes += (size_t)pl.slices * p.m * p.n * 4;
     return pl;
 }
 
@@ -546,30 +689,28 @@ hipError_t launch_mx(const MxProblem &p, const MxPlan &pl, void *workspace, hipS
     a.xs = p.xs;
     a.wq = p.wq;
     a.ws = p.ws;
-    a.y = p.y;
     a.m = (int)p.m;
     a.k = (int)p.k;
     a.n = (int)p.n;
     a.groups = (int)mx_groups(p.k);
     a.rtiles = div_up(p.m, 16);
-    const dim3 grid((unsigned)pl.grid_x, (unsigned)pl.grid_y);
+    a.ntn = div_up(p.n, kShapes[pl.shape].tn);
+    a.ntm = div_up(p.m, kShapes[pl.shape].tm);
+    a.slices = pl.slices;
+    a.per = pl.per;
+    char *w = static_cast<char *>(workspace);
     if (p.x) {
-        const int64_t units = (int64_t)a.groups * a.rtiles;
-        char *w = static_cast<char *>(workspace);
-        char *planes = w;
-        u32x2 *scales = reinterpret_cast<u32x2 *>(w + units * kDigits * kPlaneBytes);
-        uint32_t *marks = reinterpret_cast<uint32_t *>(w + units * (kDigits * kPlaneBytes + 512));
-        const int words = div_up(p.m, 32);
-        mx_clear_kernel<<<dim3(div_up(words, 256)), dim3(256), 0, stream>>>(marks, words);
-        mx_split_kernel<<<dim3((unsigned)units), dim3(256), 0, stream>>>(p.x, planes, scales, marks, a.m, a.k, a.groups, a.rtiles);
-        a.planes = planes;
-        a.scales = scales;
-        a.marks = marks;
-        mx_tile_kernel<kDigits, 2, 2><<<grid, dim3(256), 0, stream>>>(a);
-    } else {
-        mx_tile_kernel<1, 2, 2><<<grid, dim3(256), 0, stream>>>(a);
+        mx_split_kernel<<<dim3((unsigned)((int64_t)a.groups * a.rtiles)), dim3(256), 0, stream>>>(p.x, w, a.m, a.k, a.rtiles);
+        a.xq = reinterpret_cast<const uint8_t *>(w);
+        w += digits_bytes(p.m, p.k);
     }
-    return hipGetLastError();
+    a.y = pl.slices > 1 ? reinterpret_cast<float *>(w) : p.y;
+    hipError_t e = launch_shape(pl.shape, a, stream);
+    if (e == hipSuccess && pl.slices > 1) {
+        mx_sum_kernel<<<dim3((unsigned)std::min<int64_t>(2048, (p.m * p.n + 255) / 256)), dim3(256), 0, stream>>>(a, p.y);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 }  // namespace dmc

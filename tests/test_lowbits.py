@@ -82,7 +82,7 @@ def batch(**kw):
 BAD = [(cache(**c), batch(**b)) for c, b in (
     [({n: v}, {}) for n, v in (("k", 0), ("v", 0), ("k_scales", 0), ("v_scales", 0), ("k", P + 8), ("v", P + 4), ("pages", 0),
                                ("heads", 0), ("heads", 5000), ("page", 8), ("page", 48), ("page", 512), ("dim", 80), ("dim", 0))]
-    + [({}, {n: v}) for n, v in (("table", 0), ("lens", 0), ("starts", 0), ("table", P + 2), ("width", -1), ("batch", -1),
+    + [({}, {n: v}) for n, v in (("table", 0), ("lens", 0), ("starts", 0), ("table", P + 2), ("width", -1), ("width", 0), ("batch", -1),
                                  ("batch", 40000), ("max_new", -1), ("max_len", -1))])]
 
 
