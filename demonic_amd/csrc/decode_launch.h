@@ -69,6 +69,7 @@ struct KvAppend {
     const void *k, *v;      // new tokens' rows [heads][dim], ld elements apart
     int64_t k_ld, v_ld;
     bool bf16;
+    bool turn = false;      // set by the launch: whole V pages pass through LDS
 };
 hipError_t launch_kv_append(const KvAppend &p, hipStream_t stream);
 

@@ -24,31 +24,71 @@ __device__ __forceinline__ uint32_t e4m3_scale_byte(uint32_t amax) {
     return (uint32_t)max(e, 0);
 }
 
-// Magnitude bits that count for a page's scale: infs and NaNs have no code but NaN and leave it alone.
-__device__ __forceinline__ uint32_t finite_mag(float f) {
-    const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
-    return u < 0x7f800000u ? u : 0u;
-}
-
-// x 2^(127 - byte) in e4m3, to nearest even (exact scaling, one rounding); infs and NaNs become NaN.
-__device__ __forceinline__ uint32_t to_e4m3(float x, int byte) {
-    const float f = ldexpf(x, 127 - byte);
-    const uint32_t c = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f, f, 0, false) & 255u;
-    return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 0x7fu : c;
-}
-
-__device__ __forceinline__ float from_e4m3(uint32_t code) { return __builtin_amdgcn_cvt_f32_fp8((int)code, 0); }
-
 template <bool BF>
-__device__ __forceinline__ float load1(const void *p, int64_t at) {
-    if constexpr (BF) return __uint_as_float((uint32_t)static_cast<const uint16_t *>(p)[at] << 16);
-    else return static_cast<const float *>(p)[at];
+struct KvRow8 {  // 8 values of a row, any alignment of their type
+    uint32_t u[BF ? 4 : 8];
+    __device__ __forceinline__ void load(const void *p, int64_t at) {
+        if constexpr (BF) {
+            struct __attribute__((packed, aligned(2))) T { u32x4 v; };
+            const u32x4 x = reinterpret_cast<const T *>(static_cast<const uint16_t *>(p) + at)->v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = x[i];
+        } else {
+            struct __attribute__((packed, aligned(4))) T { u32x4 v, w; };
+            const T x = *reinterpret_cast<const T *>(static_cast<const float *>(p) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                u[i] = x.v[i];
+                u[4 + i] = x.w[i];
+            }
+        }
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (BF) return __uint_as_float(i & 1 ? u[i >> 1] & 0xffff0000u : u[i >> 1] << 16);
+        else return __uint_as_float(u[i]);
+    }
+    __device__ __forceinline__ uint32_t finite_max() const {  // infs and NaNs have no say in the scale
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t v = __float_as_uint(at(i)) & 0x7fffffffu;
+            m = max(m, v < 0x7f800000u ? v : 0u);
+        }
+        return m;
+    }
+    // x 2^up in e4m3, to nearest even (the scaling is exact: one rounding); infs and NaNs become NaN
+    __device__ __forceinline__ u32x2 codes(int up) const {
+        u32x2 r = {0, 0};
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            int c = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(at(4 * w), up), ldexpf(at(4 * w + 1), up), 0, false);
+            c = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(at(4 * w + 2), up), ldexpf(at(4 * w + 3), up), c, true);
+            r[w] = (uint32_t)c;
+        }
+        return r;
+    }
+};
+
+__device__ __forceinline__ uint32_t rescale4(uint32_t u, int up) {  // 4 codes times 2^up; NaN stays NaN
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, true);
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(a[0], up), ldexpf(a[1], up), 0, false);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(b[0], up), ldexpf(b[1], up), c, true);
+    return (uint32_t)c;
 }
 
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
     return v;
+}
+
+// Bytes of a dword that are among the tokens [lo, hi) at token t.
+__device__ __forceinline__ uint32_t byte_mask(int t, int lo, int hi) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m |= (t + i >= lo && t + i < hi) ? 0xffu << (8 * i) : 0u;
+    return m;
 }
 
 // ---- append -------------------------------------------------------------------
@@ -58,50 +98,123 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // with a > 0 the page keeps the tokens before them, its scale only grows, and if
 // it does their codes are rounded again (by a power of two: exact but where they
 // become subnormal).  With a == 0 the scale is the new tokens' own.
-template <bool BF>
-__global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend p) {
+//
+// An item is 4 tokens x 8 dims, read once (a thread keeps its first item between
+// the maximum and the codes; a page of more than NT items reads the others twice).
+// A K item leaves as 8 bytes per token.  V lies transposed: an item's 4 x 4 bytes
+// turn in registers into a dword per dim; a whole page passes through LDS, so that
+// it leaves as one run of 16-byte stores, a part of one by dwords and bytes.
+template <bool BF, int NT>
+__global__ __launch_bounds__(NT) void kv_append_kernel(const KvAppend p) {
+    extern __shared__ uint32_t turn[];
+    __shared__ uint32_t part[NT / 64];
     const int b = blockIdx.z >> 1, head = blockIdx.y;
     const bool is_v = blockIdx.z & 1;
-    const int D = p.c.dim, P = p.c.page;
+    const int D = p.c.dim, P = p.c.page, lgp = 31 - __clz(P), DC = D / 8;
     const int64_t start = p.b.starts[b];
     const int64_t len = p.b.lens[b];
     const int64_t count = min((int64_t)p.b.starts[b + 1] - start, (int64_t)p.b.max_new);
     const int64_t first = len - count;
     if (count <= 0 || first < 0) return;
-    const int64_t slot = first / P + blockIdx.x;
+    const int64_t slot = (first >> lgp) + blockIdx.x;
     if (slot * P >= len || slot >= p.b.width) return;
     const int64_t page = p.b.table[b * p.b.width + slot];
     if (page < 0 || page >= p.c.pages) return;
     const int a = (int)max((int64_t)0, first - slot * P), z = (int)min((int64_t)P, len - slot * P);
-    const int n = (z - a) * D;
     const int64_t ld = is_v ? p.v_ld : p.k_ld;
     const void *src = is_v ? p.v : p.k;
-    const int64_t row0 = (start + slot * P + a - first) * ld + (int64_t)head * D;
+    const int64_t row0 = (start + slot * P - first) * ld + (int64_t)head * D;  // of the page's token 0
+    const int g0 = a >> 2, items = (((z + 3) >> 2) - g0) * DC;
 
-    __shared__ uint32_t part[4];
+    KvRow8<BF> it[4];
+    auto load = [&](int i) {
+        const int t = (g0 + i / DC) * 4, c = i % DC;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) it[j].load(src, row0 + min(max(t + j, a), z - 1) * ld + c * 8);  // an edge's own row
+    };
     uint32_t mag = 0;
-    for (int i = threadIdx.x; i < n; i += 256) mag = max(mag, finite_mag(load1<BF>(src, row0 + (int64_t)(i / D) * ld + i % D)));
+    for (int i = threadIdx.x + (items - 1) / NT * NT; i >= 0; i -= NT) {  // the first item last: it stays
+        if (i >= items) continue;
+        load(i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mag = max(mag, it[j].finite_max());
+    }
     mag = wave_max(mag);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mag;
-    __syncthreads();
-    mag = max(max(part[0], part[1]), max(part[2], part[3]));
+    if constexpr (NT > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = mag;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) mag = max(mag, part[w]);
+    }
     uint8_t *scale = (is_v ? p.c.vs : p.c.ks) + page * p.c.heads + head;
     const uint32_t need = e4m3_scale_byte(mag), had = a > 0 ? *scale : 0u;
     const uint32_t byte = max(need, had);
     uint8_t *codes = (is_v ? p.c.v : p.c.k) + (page * p.c.heads + head) * (int64_t)(P * D);
-    __syncthreads();
-    if (threadIdx.x == 0) *scale = (uint8_t)byte;
-    const int ts = is_v ? 1 : D, ds = is_v ? P : 1;  // strides of a token and a dim
     if (a > 0 && byte > had) {
-        for (int i = threadIdx.x; i < a * D; i += 256) {
-            uint8_t *c = codes + (i / D) * ts + (i % D) * ds;
-            const uint32_t u = *c;
-            const uint32_t r = to_e4m3(from_e4m3(u), (int)(127 + byte - had));
-            *c = (uint8_t)((u & 0x7f) == 0x7f ? u : r);
+        // V's dwords hold tokens 4 i .. 4 i + 3 of a dim; K's tokens before a come first
+        uint32_t *w = reinterpret_cast<uint32_t *>(codes);
+        const int n = is_v ? P * D / 4 : a * D / 4;
+#pragma unroll 4
+        for (int i = threadIdx.x * 4; i < n; i += NT * 4) {
+            u32x4 u = *reinterpret_cast<const u32x4 *>(w + i);
+            const int t = (i * 4) & (P - 1);
+            if (is_v && t >= a) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t keep = is_v ? byte_mask(t + 4 * e, 0, a) : ~0u;
+                u[e] = (rescale4(u[e], (int)had - (int)byte) & keep) | (u[e] & ~keep);
+            }
+            *reinterpret_cast<u32x4 *>(w + i) = u;
+        }
+        __syncthreads();  // before the new tokens' bytes beside them
+    }
+    if (NT > 64) __syncthreads();  // every thread has read the old scale
+    if (threadIdx.x == 0) *scale = (uint8_t)byte;
+    const bool whole = is_v && a == 0 && z == P && p.turn;
+    for (int i = threadIdx.x; i < items; i += NT) {
+        if (i >= NT) load(i);
+        const int t = (g0 + i / DC) * 4, c = i % DC;
+        u32x2 q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = it[j].codes(127 - (int)byte);
+        if (!is_v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (t + j >= a && t + j < z) *reinterpret_cast<u32x2 *>(codes + (t + j) * D + c * 8) = q[j];
+            continue;
+        }
+        uint32_t d[8];  // dim e's tokens t .. t + 3
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const uint32_t lo01 = __builtin_amdgcn_perm(q[1][w], q[0][w], 0x05010400u), lo23 = __builtin_amdgcn_perm(q[3][w], q[2][w], 0x05010400u);
+            const uint32_t hi01 = __builtin_amdgcn_perm(q[1][w], q[0][w], 0x07030602u), hi23 = __builtin_amdgcn_perm(q[3][w], q[2][w], 0x07030602u);
+            d[4 * w] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+            d[4 * w + 1] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+            d[4 * w + 2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+            d[4 * w + 3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+        }
+        if (whole) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) turn[(c * 8 + e) * (P / 4 + 1) + (t >> 2)] = d[e];
+        } else if (t >= a && t + 4 <= z) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) *reinterpret_cast<uint32_t *>(codes + (c * 8 + e) * P + t) = d[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t + j >= a && t + j < z) codes[(c * 8 + e) * P + t + j] = (uint8_t)(d[e] >> (8 * j));
         }
     }
-    for (int i = threadIdx.x; i < n; i += 256)
-        codes[(a + i / D) * ts + (i % D) * ds] = (uint8_t)to_e4m3(load1<BF>(src, row0 + (int64_t)(i / D) * ld + i % D), (int)byte);
+    if (whole) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < P * D / 16; i += NT) {
+            const int dim = i * 16 >> lgp, w = (i * 4) & (P / 4 - 1);
+            const uint32_t *s = turn + dim * (P / 4 + 1) + w;
+            *reinterpret_cast<u32x4 *>(codes + i * 16) = u32x4{s[0], s[1], s[2], s[3]};
+        }
+    }
 }
 
 // ---- attention ------------------------------------------------------------------
@@ -124,6 +237,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend p) {
 // of 16), and are the k positions that the V' operand wants from one 16-byte read
 // of a dim's tokens.
 constexpr int kStep = 64;  // tokens per wave and step
+constexpr int kMaxSplits = 256;  // workgroups along one sequence
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {  // 8 codes to bf16
@@ -163,14 +277,6 @@ __device__ __forceinline__ float ror_add(float v) {  // over columns c, c + 4, c
     return v;
 }
 
-// Bytes of a dword that are among the token range [lo, hi) at token t.
-__device__ __forceinline__ uint32_t byte_mask(int t, int lo, int hi) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m |= (t + i >= lo && t + i < hi) ? 0xffu << (8 * i) : 0u;
-    return m;
-}
-
 // Bytes 0x01 where a code is NaN (0x7f or 0xff).
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {
     return (((v & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
@@ -208,10 +314,11 @@ struct KvPart {
     float *ml; // [splits][rows][2]
 };
 
-// Workgroups (column tile, token split), heads, sequences; 4 waves take steps of 64 tokens in turn, each
-// with the next step's codes on their way to registers while it works on this one's.
+// Workgroups (column tile, token split), heads, sequences; 4 waves take steps of 64 tokens in turn.  A step's V is
+// on its way to registers while its scores are formed, the next step's K from then on (into the registers
+// that held this one's), so that each wave has 8 to 16 KB in flight without a second set of registers.
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const KvPart part, int splits, int chunk,
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const KvAttend p, const KvPart part, int splits, int chunk,
                                                       int row_tiles, int64_t rows_total) {
     constexpr int R = BF ? 16 : 4;      // query rows per column tile
     constexpr int KS = D / 32;          // MFMA steps over dims
@@ -252,39 +359,23 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
         return t < most ? id : -1;
     };
     auto safe = [&](int id) -> int64_t { return id >= 0 && id < p.c.pages ? id : 0; };
-    struct Codes {
-        u32x4 v[DT];
-        u32x4 k[WIDE ? 4 * KP : 1];
-        u32x2 k8[WIDE ? 1 : 4 * KP];
-        uint32_t ks, vs;
-        bool in;
-    };
-    // the pages of the 16 tokens that a K row (its r / 4) and this lane's own tokens lie in
-    auto load = [&](Codes &c, int t0, int pk, int pv) {
-        const int tk = t0 + 16 * (col >> 2), tv = t0 + 16 * quad;
-        const uint8_t *kp = p.c.k + (safe(pk) * p.c.heads + head) * page_bytes + ((tk & (P - 1)) + (col & 3)) * D;
-        const uint8_t *vp = p.c.v + (safe(pv) * p.c.heads + head) * page_bytes + col * P + (tv & (P - 1));
+    u32x4 kw[WIDE ? 4 * KP : 1];
+    u32x2 k8[WIDE ? 1 : 4 * KP];
+    // pk: the page of the 16 tokens that this lane's K rows (r / 4) lie in, pv: of this lane's own tokens
+    auto load_k = [&](int t0, int pk) {
+        const uint8_t *kp = p.c.k + (safe(pk) * p.c.heads + head) * page_bytes + (((t0 + 16 * (col >> 2)) & (P - 1)) + (col & 3)) * D;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
-                if constexpr (WIDE) c.k[j * KP + i] = *reinterpret_cast<const u32x4 *>(kp + j * 4 * D + i * 64 + quad * 16);
-                else c.k8[j * KP + i] = *reinterpret_cast<const u32x2 *>(kp + j * 4 * D + i * 32 + quad * 8);
+                if constexpr (WIDE) kw[j * KP + i] = *reinterpret_cast<const u32x4 *>(kp + j * 4 * D + i * 64 + quad * 16);
+                else k8[j * KP + i] = *reinterpret_cast<const u32x2 *>(kp + j * 4 * D + i * 32 + quad * 8);
             }
-        c.ks = p.c.ks[safe(pv) * p.c.heads + head];
-        c.vs = p.c.vs[safe(pv) * p.c.heads + head];
-        c.in = pv >= 0 && pv < p.c.pages;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) c.v[d] = *reinterpret_cast<const u32x4 *>(vp + d * 16 * P);
     };
-    Codes now;
-    int pk, pv;
-    {
-        const int t0 = from + wave * kStep;
-        load(now, t0, page_of(t0 + 16 * (col >> 2)), page_of(t0 + 16 * quad));
-        pk = page_of(t0 + 4 * kStep + 16 * (col >> 2));
-        pv = page_of(t0 + 4 * kStep + 16 * quad);
-    }
+    const int first = from + wave * kStep, tko = 16 * (col >> 2), tvo = 16 * quad;
+    int pv = page_of(first + tvo), pk = page_of(first + 4 * kStep + tko), pv_next = page_of(first + 4 * kStep + tvo);
+    load_k(first, page_of(first + tko));
+    uint32_t ksb = p.c.ks[safe(pv) * p.c.heads + head], vsb = p.c.vs[safe(pv) * p.c.heads + head];
 
     u32x4 qf[KS];
 #pragma unroll
@@ -307,13 +398,14 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
     float m = -INFINITY, sum = 0.0f;
     uint32_t nans = 0;
 
-    for (int t0 = from + wave * kStep; t0 < to; t0 += 4 * kStep) {
-        Codes next;
-        load(next, t0 + 4 * kStep, pk, pv);  // past the end: some page's codes, not used
-        pk = page_of(t0 + 8 * kStep + 16 * (col >> 2));
-        pv = page_of(t0 + 8 * kStep + 16 * quad);
-        const int tv = t0 + 16 * quad;
-        const float ks = e8m0(now.ks) * scale, vs = e8m0(now.vs);
+    for (int t0 = first; t0 < to; t0 += 4 * kStep) {
+        const int tv = t0 + tvo;
+        const bool in = pv >= 0 && pv < p.c.pages;
+        u32x4 vw[DT];
+        const uint8_t *vp = p.c.v + (safe(pv) * p.c.heads + head) * page_bytes + col * P + (tv & (P - 1));
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4 *>(vp + d * 16 * P);
+        const float ks = e8m0(ksb) * scale, vs = e8m0(vsb);
         float s[16];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -321,20 +413,27 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
                 if constexpr (WIDE) {
-                    const u32x4 w = now.k[j * KP + i];
+                    const u32x4 w = kw[j * KP + i];
                     c = mma(widen8(w[0], w[1]), qf[2 * i], c);
                     c = mma(widen8(w[2], w[3]), qf[2 * i + 1], c);
                 } else {
-                    const u32x2 w = now.k8[j * KP + i];
+                    const u32x2 w = k8[j * KP + i];
                     c = mma(widen8(w[0], w[1]), qf[i], c);
                 }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[4 * j + i] = c[i];
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(t0 + 4 * kStep, pk);  // past the end: some page's codes, not used
+        pv = pv_next;
+        ksb = p.c.ks[safe(pv) * p.c.heads + head];
+        vsb = p.c.vs[safe(pv) * p.c.heads + head];
+        pk = page_of(t0 + 8 * kStep + tko);
+        pv_next = page_of(t0 + 8 * kStep + tvo);
         const bool whole = t0 >= see_lo && t0 >= t_hi - (p.window > 0 ? p.window - 1 : INT32_MAX - 1) &&
                            t0 + kStep - 1 <= t_lo && t0 + kStep <= most;
-        const bool every = __builtin_amdgcn_ballot_w64(!now.in) == 0 && whole;  // nothing masked in this step
+        const bool every = __builtin_amdgcn_ballot_w64(!in) == 0 && whole;  // nothing masked in this step
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             if constexpr (!BF) s[i] = ror_add(s[i]);
@@ -342,18 +441,18 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
         }
         if (!every) {
             // codes that no row sees read as zero, and so do NaN codes, for now (nan_dims)
-            const int lo = now.in ? vis_lo - tv : 16, hi = vis_hi - tv;
+            const int lo = in ? vis_lo - tv : 16, hi = vis_hi - tv;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
             uint32_t keep[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) keep[i] = byte_mask(tv + 4 * i, see_lo, now.in ? see_hi : 0);
+            for (int i = 0; i < 4; ++i) keep[i] = byte_mask(tv + 4 * i, see_lo, in ? see_hi : 0);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t u = now.v[d][i] & keep[i], bad = nan_bytes(u);
-                    now.v[d][i] = u & ~(bad * 0xffu);
+                    const uint32_t u = vw[d][i] & keep[i], bad = nan_bytes(u);
+                    vw[d][i] = u & ~(bad * 0xffu);
                     nans |= bad;
                 }
         }
@@ -390,11 +489,10 @@ __global__ __launch_bounds__(256) void kv_rows_kernel(const KvAttend p, const Kv
             }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-            const u32x4 v = now.v[d];
+            const u32x4 v = vw[d];
             o[d] = mma(widen8(v[0], v[1]), pf[0], o[d]);
             o[d] = mma(widen8(v[2], v[3]), pf[1], o[d]);
         }
-        now = next;
     }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
@@ -799,19 +897,34 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvAttend p, const Kv
     const int span = see_hi - (see_lo & ~(kStep - 1));
     const int used = max(1, min(splits, (span + chunk - 1) / chunk));
     const int64_t at = ((int64_t)b * p.b.max_new + i) * p.q_heads + h, step = rows_total * p.q_heads;
+    // the splits' weights once, then their sums with independent loads
+    __shared__ float f[kMaxSplits];
     float top = -INFINITY;
     for (int s = lane; s < used; s += 64) top = fmaxf(top, part.ml[(at + s * step) * 2]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     const float ref = top == -INFINITY ? 0.0f : top;
-    float val[4] = {0, 0, 0, 0}, tot = 0.0f;
-#pragma unroll 4
-    for (int s = wave; s < used; s += 4) {
-        const float f = __builtin_amdgcn_exp2f(part.ml[(at + s * step) * 2] - ref);
-        tot += f * part.ml[(at + s * step) * 2 + 1];
+    float tot = 0.0f;
+    for (int s = threadIdx.x; s < used; s += 256) {
+        f[s] = __builtin_amdgcn_exp2f(part.ml[(at + s * step) * 2] - ref);
+        tot += f[s] * part.ml[(at + s * step) * 2 + 1];
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (lane + 64 * j < D) val[j] += f * part.o[(at + s * step) * D + lane + 64 * j];
+    for (int d = 32; d; d >>= 1) tot += __shfl_xor(tot, d);
+    __syncthreads();
+    float val[4] = {0, 0, 0, 0};
+    const float *po = part.o + at * D + lane;
+    for (int s = wave; s < used; s += 32) {
+        float v[8][4];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[u][j] = s + 4 * u < used && lane + 64 * j < D ? po[(s + 4 * u) * step * D + 64 * j] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) val[j] += (s + 4 * u < used ? f[s + 4 * u] : 0.0f) * v[u][j];
     }
     __shared__ float vals[4][256], tots[4];
 #pragma unroll
@@ -876,11 +989,19 @@ hipError_t attend(const KvAttend &p, const KvPlan &pl, void *workspace, hipStrea
 
 bool kv_dim_served(int64_t dim) { return dim == 64 || dim == 96 || dim == 128 || dim == 256; }
 
-hipError_t launch_kv_append(const KvAppend &p, hipStream_t stream) {
-    const int slots = (p.b.max_new + p.c.page - 1) / p.c.page + 1;
-    const dim3 grid((unsigned)slots, (unsigned)p.c.heads, (unsigned)p.b.batch * 2);
-    if (p.bf16) kv_append_kernel<true><<<grid, dim3(256), 0, stream>>>(p);
-    else kv_append_kernel<false><<<grid, dim3(256), 0, stream>>>(p);
+hipError_t launch_kv_append(const KvAppend &args, hipStream_t stream) {
+    KvAppend p = args;
+    const int P = p.c.page, D = p.c.dim;
+    const dim3 grid((unsigned)((p.b.max_new + 2 * P - 2) / P), (unsigned)p.c.heads, (unsigned)p.b.batch * 2);
+    // few tokens are one wave's work (up to 8 of 4 x 8 values in 64 threads): no barrier between waves
+    const bool few = p.b.max_new <= 4;
+    const size_t lds = (size_t)D * (P / 4 + 1) * 4;
+    p.turn = !few && lds <= 64 * 1024 - 64;
+    const size_t use = p.turn ? lds : 0;
+    if (few && p.bf16) kv_append_kernel<true, 64><<<grid, dim3(64), use, stream>>>(p);
+    else if (few) kv_append_kernel<false, 64><<<grid, dim3(64), use, stream>>>(p);
+    else if (p.bf16) kv_append_kernel<true, 256><<<grid, dim3(256), use, stream>>>(p);
+    else kv_append_kernel<false, 256><<<grid, dim3(256), use, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -896,7 +1017,7 @@ KvPlan plan_kv(const KvAttend &p, int num_cus) {
     const int64_t units = std::max<int64_t>(1, (span + unit - 1) / unit);
     const int64_t want = std::max<int64_t>(1, (pl.kind ? 2 : 8) * num_cus / std::max<int64_t>(1, tiles));
     // steps per workgroup: a split of few costs more in its partial results than it saves
-    const int64_t per = std::max<int64_t>((units + want - 1) / want, pl.kind ? 8 : 4);
+    const int64_t per = std::max<int64_t>((units + want - 1) / want, std::max<int64_t>(pl.kind ? 8 : 4, (units + kMaxSplits - 1) / kMaxSplits));
     pl.chunk = (int)(per * unit);
     pl.splits = (int)((units + per - 1) / per);
     if (pl.splits > 1)
