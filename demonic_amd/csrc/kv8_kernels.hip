@@ -10,6 +10,8 @@ namespace dmc {
 namespace {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 // The f32 of 2^(byte - 127); 255 is NaN, 0 is 2^-127, a subnormal.
@@ -70,7 +72,6 @@ struct KvRow8 {  // 8 values of a row, any alignment of their type
 };
 
 __device__ __forceinline__ uint32_t rescale4(uint32_t u, int up) {  // 4 codes times 2^up; NaN stays NaN
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
     const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, true);
     int c = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(a[0], up), ldexpf(a[1], up), 0, false);
     c = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(b[0], up), ldexpf(b[1], up), c, true);
@@ -240,12 +241,12 @@ constexpr int kStep = 64;  // tokens per wave and step
 constexpr int kMaxSplits = 256;  // workgroups along one sequence
 constexpr float kLog2e = 1.44269504088896340736f;
 
-__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi) {  // 8 codes to bf16
+__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float scale) {  // 8 codes times a power of two, to bf16
     u32x4 r;
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
     return r;
 }
 
@@ -302,6 +303,11 @@ __device__ __forceinline__ uint64_t nan_dims(const KvAttend &p, const int32_t *t
     return bits;
 }
 
+__device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i's 16 bytes to l + 16 i
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
+                                     (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
+}
+
 __device__ __forceinline__ float quads_max(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
@@ -356,9 +362,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
     const int64_t page_bytes = (int64_t)P * D;
     auto page_of = [&](int t) -> int {  // no branch: past the table, its last entry is read and not taken
         const int id = table[min(t, most - 1) >> lgp];
-        return t < most ? id : -1;
+        return t < most && (uint32_t)id < (uint32_t)p.c.pages ? id : -1;
     };
-    auto safe = [&](int id) -> int64_t { return id >= 0 && id < p.c.pages ? id : 0; };
+    auto safe = [&](int id) -> int64_t { return max(id, 0); };
     u32x4 kw[WIDE ? 4 * KP : 1];
     u32x2 k8[WIDE ? 1 : 4 * KP];
     // pk: the page of the 16 tokens that this lane's K rows (r / 4) lie in, pv: of this lane's own tokens
@@ -400,12 +406,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
 
     for (int t0 = first; t0 < to; t0 += 4 * kStep) {
         const int tv = t0 + tvo;
-        const bool in = pv >= 0 && pv < p.c.pages;
+        const bool in = pv >= 0;
         u32x4 vw[DT];
         const uint8_t *vp = p.c.v + (safe(pv) * p.c.heads + head) * page_bytes + col * P + (tv & (P - 1));
 #pragma unroll
         for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4 *>(vp + d * 16 * P);
-        const float ks = e8m0(ksb) * scale, vs = e8m0(vsb);
+        const float ks = e8m0(ksb) * scale, vs = in ? e8m0(vsb) : 1.0f;  // an absent page's byte may be any
         float s[16];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -414,11 +420,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
             for (int i = 0; i < KP; ++i) {
                 if constexpr (WIDE) {
                     const u32x4 w = kw[j * KP + i];
-                    c = mma(widen8(w[0], w[1]), qf[2 * i], c);
-                    c = mma(widen8(w[2], w[3]), qf[2 * i + 1], c);
+                    c = mma(widen8(w[0], w[1], 1.0f), qf[2 * i], c);
+                    c = mma(widen8(w[2], w[3], 1.0f), qf[2 * i + 1], c);
                 } else {
                     const u32x2 w = k8[j * KP + i];
-                    c = mma(widen8(w[0], w[1]), qf[i], c);
+                    c = mma(widen8(w[0], w[1], 1.0f), qf[i], c);
                 }
             }
 #pragma unroll
@@ -476,7 +482,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
         for (int i = 0; i < 16; ++i) {
             s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
             add += s[i];
-            s[i] *= vs;
         }
         sum += add;
         u32x4 pf[2];
@@ -490,8 +495,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const u32x4 v = vw[d];
-            o[d] = mma(widen8(v[0], v[1]), pf[0], o[d]);
-            o[d] = mma(widen8(v[2], v[3]), pf[1], o[d]);
+            o[d] = mma(widen8(v[0], v[1], vs), pf[0], o[d]);
+            o[d] = mma(widen8(v[2], v[3], vs), pf[1], o[d]);
         }
     }
     sum += __shfl_xor(sum, 16);
@@ -557,37 +562,47 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
 // ---- attention, tiles of query rows ----------------------------------------------
 //
 // Prompts: a workgroup of 4 waves owns 64 * CT query rows of one cache head (tokens x
-// the head's group of query heads) and walks the tokens 64 at a time.  The codes go to
-// LDS as they are, without passing through registers, one step ahead; every wave widens
-// them for its own CT column tiles.  f32 rows take one MFMA per term of q (3) and of
-// the weights (3) instead of a column per term, so that a weight is computed once.
+// the head's group of query heads) and walks the tokens 64 at a time.
 //
-// 16-byte pieces of a K row (a dim's tokens of V) are stored in an order that depends on
-// the row, so that the 8 lanes that read at a time meet different banks.
+// What bounds it is vector instructions beside the MFMAs, so the widening of codes is
+// kept out of the waves' way:
+//  - codes go to LDS as they are, without passing through registers, a step ahead;
+//  - bf16 rows: the scaled MFMA takes K's codes themselves against q as two e4m3 terms
+//    (4 bits each of the row's 8, after a power of two for the row): as many MFMA
+//    cycles as one bf16 term, and no widening.  Elements below 2^-10 of their row's
+//    largest lose bits, at most 2^-18 of that one;
+//  - f32 rows: K widens in each wave, one MFMA per bf16 term of q (3);
+//  - V widens once for the workgroup, with its scale, on its way from one LDS buffer to
+//    another; a weight enters in one bf16 term (f32: 3);
+//  - the weights' sum is one more row of the product, V' = 1: sums of what was used.
+//
+// 16-byte pieces lie in an order that depends on their row, so that the 16 lanes that
+// read at a time meet different banks.
 template <int D>
 struct KvTile {
-    static constexpr int KC = D / 16;                     // pieces of a K row
-    static constexpr int K_BYTES = kStep * D, BYTES = 2 * kStep * D;
+    static constexpr int KC = D / 16;                        // pieces of a K row
+    static constexpr int RAW = kStep * D;                    // bytes of one side's codes
     static constexpr int PASSES = (kStep * KC + 255) / 256;  // pieces per thread and side
+    static constexpr int LDS = 2 * 2 * RAW + 2 * RAW;        // two stages of codes, V in bf16
     static __device__ __forceinline__ int k_slot(int t, int c) {
-        return KC == 6 ? c : c ^ (((t & 3) | ((t >> 2) & 4)) & (KC >= 8 ? 7 : 3));
+        if (KC == 16) return c ^ ((t & 3) | ((t >> 2) & 12));
+        if (KC == 8) return c ^ (((t >> 1) & 1) | ((t >> 3) & 6));
+        if (KC == 4) return c ^ ((t >> 4) & 3);
+        return c;
     }
-    static __device__ __forceinline__ int v_slot(int d, int c) { return c ^ ((d >> 1) & 3); }
 };
 
-__device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i's 16 bytes to l + 16 i
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
-                                     (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
-}
-
-template <int D, bool BF, int CT>
-__global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(const KvAttend p, const KvPart part, int splits, int chunk,
-                                                          int row_tiles, int64_t rows_total) {
+// UP: pages hold 64 tokens or more, so that a step lies in one, the same for all lanes.
+template <int D, bool BF, int CT, bool UP>
+__global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(const KvAttend p, const KvPart part, int splits,
+                                                                               int chunk, int row_tiles, int64_t rows_total) {
     using T = KvTile<D>;
-    constexpr int PL = BF ? 1 : 3;  // terms of q and of the weights
-    constexpr int KS = D / 32, DT = D / 16, LB = D / 4, R = 64 * CT;
-    __shared__ __attribute__((aligned(16))) char lds[2][T::BYTES];
+    constexpr int PL = BF ? 1 : 3;  // bf16 terms of the weights, and of q where it is f32
+    constexpr int KS = D / 32, DT = D / 16, R = 64 * CT;
+    constexpr int QC = (D + 127) / 128, QT = D == 64 ? 1 : 2;  // bf16 rows: MFMAs over dims, over terms (64: both in one)
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ int nans;
+    char *const vbuf = lds + 4 * T::RAW;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int col = lane & 15, quad = lane >> 4;
     // heads turn fastest: with 8 of them each XCD keeps one head's codes in its L2
@@ -608,7 +623,10 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
     const int to = split == splits - 1 ? see_hi : min(from + chunk, see_hi);
     if (split > 0 && from >= see_hi) return;
 
-    u32x4 qf[CT][PL][KS];
+    // ---- q: e4m3 terms (bf16 rows) or bf16 terms (f32 rows), and the rows' limits
+    i32x8 q8[BF ? CT : 1][QT][QC];
+    u32x4 q16[BF ? 1 : CT][PL][KS];
+    float qscale[CT];
     int vis_lo[CT], vis_hi[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -616,203 +634,248 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
         const int pos = len - count + my / group;
         vis_lo[c] = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         vis_hi[c] = min(pos + 1, most);
-        const int64_t q0 = (start + my / group) * p.q_ld + (int64_t)(head * group + my % group) * D + quad * LB;
+        const int64_t q0 = (start + my / group) * p.q_ld + (int64_t)(head * group + my % group) * D;
+        if constexpr (BF) {
+            // dims 128 h + 32 quad on; 64 dims: quads 0 and 1 the first term, 2 and 3 the second; 96: quad 3 none
+            KvRow8<true> x[QC][4];
+            uint32_t big = 0;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            if constexpr (BF) {
-                struct __attribute__((packed, aligned(2))) T8 { u32x4 v; };
-                qf[c][0][s] = reinterpret_cast<const T8 *>(static_cast<const uint16_t *>(p.q) + q0 + s * 8)->v;
-            } else {
-                const float *f = static_cast<const float *>(p.q) + q0 + s * 8;
+            for (int h = 0; h < QC; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int at = D == 64 ? (quad & 1) * 32 : D == 96 ? min(quad, 2) * 32 : h * 128 + quad * 32;
+                    x[h][i].load(p.q, q0 + at + i * 8);
+                    big = max(big, x[h][i].finite_max());
+                }
+            const uint32_t byte = e4m3_scale_byte(__float_as_uint(quads_max(__uint_as_float(big))));
+            qscale[c] = e8m0(byte);
+#pragma unroll
+            for (int h = 0; h < QC; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int t = 0; t < PL; ++t) qf[c][t][s][i] = pair_cut(term_of(f[2 * i], t), term_of(f[2 * i + 1], t));
+                    for (int w = 0; w < 2; ++w) {
+                        int first = 0, second = 0;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const float f0 = ldexpf(x[h][i].at(4 * w + 2 * half), 127 - (int)byte);
+                            const float f1 = ldexpf(x[h][i].at(4 * w + 2 * half + 1), 127 - (int)byte);
+                            const int r = __builtin_amdgcn_cvt_pk_fp8_f32(f0, f1, 0, false);
+                            const f32x2 v = __builtin_amdgcn_cvt_pk_f32_fp8(r, false);
+                            const int e = __builtin_amdgcn_cvt_pk_fp8_f32(f0 - v[0], f1 - v[1], 0, false);
+                            first |= (r & 0xffff) << (16 * half);
+                            second |= (e & 0xffff) << (16 * half);
+                        }
+                        if (D == 96 && quad == 3) first = second = 0;
+                        if constexpr (QT == 1) {
+                            q8[c][0][h][2 * i + w] = quad >> 1 ? second : first;
+                        } else {
+                            q8[c][0][h][2 * i + w] = first;
+                            q8[c][1][h][2 * i + w] = second;
+                        }
+                    }
+        } else {
+            qscale[c] = 1.0f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const float *f = static_cast<const float *>(p.q) + q0 + quad * (D / 4) + s * 8;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int t = 0; t < PL; ++t) q16[c][t][s][i] = pair_cut(term_of(f[2 * i], t), term_of(f[2 * i + 1], t));
             }
         }
     }
 
+    // ---- where codes come from: pieces of a step, per thread
     const int32_t *table = p.b.table + (int64_t)b * p.b.width;
     const float scale = p.scale * kLog2e;
-    const int64_t page_bytes = (int64_t)P * D;
+    const int64_t page_bytes = (int64_t)P * D, stride = page_bytes * p.c.heads;
+    const uint8_t *const kh = p.c.k + head * page_bytes, *const vh = p.c.v + head * page_bytes;
     auto page_of = [&](int t) -> int {  // no branch: past the table, its last entry is read and not taken
         const int id = table[min(t, most - 1) >> lgp];
-        return t < most ? id : -1;
+        return t < most && (uint32_t)id < (uint32_t)p.c.pages ? id : -1;
     };
-    auto safe = [&](int id) -> int64_t { return id >= 0 && id < p.c.pages ? id : 0; };
-
-    // This thread's pieces of a step: K token rows kt[], V's 16 tokens vc.
-    int kt[T::PASSES], kc[T::PASSES], vd[T::PASSES];
-    const int vslot = threadIdx.x & 3, vc = vslot ^ ((threadIdx.x >> 3) & 3);
+    int kt[T::PASSES], ko[T::PASSES], vo[T::PASSES];  // token row; offsets within the step of a K and a V piece
+    const int vc = threadIdx.x & 3;                   // a V piece's 16 tokens
 #pragma unroll
     for (int i = 0; i < T::PASSES; ++i) {
         const int at = i * 256 + threadIdx.x;
         kt[i] = at / T::KC;
-        kc[i] = T::k_slot(kt[i], at % T::KC);
-        vd[i] = at >> 2;
+        ko[i] = kt[i] * D + T::k_slot(kt[i], at % T::KC) * 16;
+        vo[i] = (at >> 2) * P + vc * 16;
     }
-    int kid[T::PASSES], vid;
+    constexpr int IDS = UP ? 1 : T::PASSES;
+    int kid[IDS], vid;
     auto ids = [&](int t0) {
+        if constexpr (UP) {
+            kid[0] = vid = page_of(t0);
+        } else {
 #pragma unroll
-        for (int i = 0; i < T::PASSES; ++i) kid[i] = kt[i] < kStep ? page_of(t0 + kt[i]) : -1;
-        vid = page_of(t0 + 16 * vc);
+            for (int i = 0; i < IDS; ++i) kid[i] = page_of(t0 + min(kt[i], kStep - 1));
+            vid = page_of(t0 + 16 * vc);
+        }
+    };
+    auto live = [&](int i) {  // a last pass may be the first waves' only
+        return !(kStep * T::KC % 256) || i < T::PASSES - 1 || wave * 64 < kStep * T::KC % 256;
     };
     auto fetch = [&](int t0, char *buf) {
+        const int in = t0 & (P - 1);
 #pragma unroll
         for (int i = 0; i < T::PASSES; ++i) {
-            if (kStep * T::KC % 256 && i == T::PASSES - 1 && wave * 64 >= kStep * T::KC % 256) break;
-            const uint8_t *k = p.c.k + (safe(kid[i]) * p.c.heads + head) * page_bytes + ((t0 + kt[i]) & (P - 1)) * D + kc[i] * 16;
+            if (!live(i)) break;
+            const uint8_t *k = UP ? kh + max(kid[0], 0) * stride + in * D + ko[i]
+                                  : kh + max(kid[UP ? 0 : i], 0) * stride + (((t0 + kt[i]) & (P - 1)) - kt[i]) * D + ko[i];
             lds_copy16(k, buf + (i * 256 + wave * 64) * 16);
         }
-        const uint8_t *v = p.c.v + (safe(vid) * p.c.heads + head) * page_bytes + ((t0 + 16 * vc) & (P - 1));
+        const uint8_t *v = vh + max(vid, 0) * stride + (UP ? in : ((t0 + 16 * vc) & (P - 1)) - 16 * vc);
 #pragma unroll
         for (int i = 0; i < T::PASSES; ++i) {
-            if (kStep * T::KC % 256 && i == T::PASSES - 1 && wave * 64 >= kStep * T::KC % 256) break;
-            lds_copy16(v + vd[i] * P, buf + T::K_BYTES + (i * 256 + wave * 64) * 16);
+            if (!live(i)) break;
+            lds_copy16(v + vo[i], buf + T::RAW + (i * 256 + wave * 64) * 16);
         }
     };
 
-    f32x4 o[CT][DT];
-    float m[CT], sum[CT];
+    f32x4 o[CT][DT], total[CT];
+    float m[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         m[c] = -INFINITY;
-        sum[c] = 0.0f;
+        total[c] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[c][d] = f32x4{0, 0, 0, 0};
     }
-    // where this lane's K row pieces (tokens 4 j on, piece i by its low bits) and V pieces lie
+    // this lane's K pieces (token rows 4 j on) and V pieces
     const int k_tok = 16 * (col >> 2) + (col & 3);
-    const int k_at = k_tok * D, k_piece = KS % 2 == 0 ? T::k_slot(k_tok, quad * (KS / 2)) * 16 : 0;
-    const int v_at = (col * 4 + T::v_slot(col, quad)) * 16;
+    const int k_piece = BF ? (D == 64 ? 2 * (quad & 1) : D == 96 ? min(2 * quad, 4) : 2 * quad) : (KS % 2 == 0 ? quad * (KS / 2) : 0);
+    const int k_at = k_tok * D, k_first = T::k_slot(k_tok, k_piece) * 16;
+    const int v_at = col * 128 + (((2 * quad) ^ ((col >> 1) & 7)) * 16);
     int buf = 0;
     if (threadIdx.x == 0) nans = 0;
     if (from < to) {
         ids(from);
-        fetch(from, lds[0]);
-        ids(from + kStep);
+        fetch(from, lds);
     }
-    // this lane's 16 tokens: their page and its scales, a step ahead of their use
-    int own = page_of(from + 16 * quad), own_next = page_of(from + kStep + 16 * quad);
-    uint32_t ksb = p.c.ks[safe(own) * p.c.heads + head], vsb = p.c.vs[safe(own) * p.c.heads + head];
+    // a step ahead: the scales of the V pieces and of this lane's own 16 tokens, and whether these are there
+    int vid_now = from < to ? vid : -1, own = UP ? vid_now : from < to ? page_of(from + 16 * quad) : -1;
+    uint32_t vsb = p.c.vs[max(vid_now, 0) * (int64_t)p.c.heads + head], ksb = p.c.ks[max(own, 0) * (int64_t)p.c.heads + head];
+    if (from < to) ids(from + kStep);
     for (int t0 = from; t0 < to; t0 += kStep) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (t0 + kStep < to) fetch(t0 + kStep, lds[buf ^ 1]);
+        char *const raw = lds + buf * (2 * T::RAW);
+        if (t0 + kStep < to) fetch(t0 + kStep, lds + (buf ^ 1) * (2 * T::RAW));
+        const bool in = own >= 0, v_in = vid_now >= 0;
+        const float ks = e8m0(ksb) * scale, vs = v_in ? e8m0(vsb) : 1.0f;  // an absent page's byte may be any
+        vid_now = vid;
+        own = UP ? vid : page_of(t0 + kStep + 16 * quad);
+        vsb = p.c.vs[max(vid_now, 0) * (int64_t)p.c.heads + head];
+        ksb = p.c.ks[max(own, 0) * (int64_t)p.c.heads + head];
         ids(t0 + 2 * kStep);
-        const bool in = own >= 0 && own < p.c.pages;
-        const float ks = e8m0(ksb) * scale;
-        const uint32_t vb = vsb;
-        own = own_next;
-        own_next = page_of(t0 + 2 * kStep + 16 * quad);
-        ksb = p.c.ks[safe(own) * p.c.heads + head];
-        vsb = p.c.vs[safe(own) * p.c.heads + head];
         const int tv = t0 + 16 * quad;
         const bool whole = t0 >= see_lo && t0 >= t_hi - (p.window > 0 ? p.window - 1 : INT32_MAX - 1) &&
                            t0 + kStep - 1 <= t_lo && t0 + kStep <= most;
         const bool every = __builtin_amdgcn_ballot_w64(!in) == 0 && whole;  // nothing masked in this step
-        if (!every) {
-            // V codes that no row sees read as zero, and so do NaN codes, for now (nan_dims); every wave
-            // sees the same four pages, so the whole workgroup is here
-            const int t = t0 + 16 * vc;
-            const int id = page_of(t);
-            const int hi = id >= 0 && id < p.c.pages ? see_hi : 0;
-            uint32_t bad = 0;
+
+        // V to bf16
 #pragma unroll
-            for (int i = 0; i < T::PASSES; ++i) {
-                if (i * 256 + (int)threadIdx.x >= kStep * T::KC) break;
-                uint32_t *v = reinterpret_cast<uint32_t *>(lds[buf] + T::K_BYTES + (i * 256 + threadIdx.x) * 16);
+        for (int i = 0; i < T::PASSES; ++i) {
+            if (!live(i)) break;
+            const int at = i * 256 + threadIdx.x, dim = at >> 2;
+            u32x4 v = *reinterpret_cast<const u32x4 *>(raw + T::RAW + at * 16);
+            if (!whole || !v_in) {
+                // codes that no row sees read as zero, and so do NaN codes, for now (nan_dims)
+                const int tt = t0 + 16 * vc, hi = v_in ? see_hi : 0;
+                uint32_t bad = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t u = v[e] & byte_mask(t + 4 * e, see_lo, hi), n = nan_bytes(u);
+                    const uint32_t u = v[e] & byte_mask(tt + 4 * e, see_lo, hi), n = nan_bytes(u);
                     bad |= n;
                     v[e] = u & ~(n * 0xffu);
                 }
+                if (bad) nans = 1;
             }
-            if (bad) nans = 1;
-            __syncthreads();
+            char *w = vbuf + dim * 128;
+            const int key = (dim >> 1) & 7;
+            *reinterpret_cast<u32x4 *>(w + ((2 * vc) ^ key) * 16) = widen8(v[0], v[1], vs);
+            *reinterpret_cast<u32x4 *>(w + ((2 * vc + 1) ^ key) * 16) = widen8(v[2], v[3], vs);
         }
-        const char *kb = lds[buf] + k_at, *vl = lds[buf] + T::K_BYTES + v_at;
 
-        float s[CT][16];
+        // scores
+        f32x4 s[CT][4];
+        const char *kb = raw + k_at;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (j) __builtin_amdgcn_sched_barrier(0);
-            u32x2 w[KS];
-            if constexpr (KS % 2 == 0) {
 #pragma unroll
-                for (int i = 0; i < KS / 2; ++i) {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (k_piece ^ (i * 16)));
-                    w[2 * i] = u32x2{x[0], x[1]};
-                    w[2 * i + 1] = u32x2{x[2], x[3]};
+            for (int c = 0; c < CT; ++c) s[c][j] = f32x4{0, 0, 0, 0};
+            if constexpr (BF) {
+#pragma unroll
+                for (int h = 0; h < QC; ++h) {
+                    u32x4 lo = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + ((k_first ^ (h * 128)))),
+                          hi = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (KvTile<D>::KC == 6 ? k_first + 16 : k_first ^ (h * 128 + 16)));
+                    if (D == 96 && quad == 3) lo = hi = u32x4{0, 0, 0, 0};
+                    const i32x8 a = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+#pragma unroll
+                    for (int t = QT - 1; t >= 0; --t)
+#pragma unroll
+                        for (int c = 0; c < CT; ++c)
+                            s[c][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q8[c][t][h], s[c][j], 0, 0, 0, 127, 0, 127);
                 }
             } else {
+                u32x2 w[KS];
+                if constexpr (KS % 2 == 0) {
 #pragma unroll
-                for (int i = 0; i < KS; ++i) w[i] = *reinterpret_cast<const u32x2 *>(kb + j * 4 * D + quad * LB + i * 8);
+                    for (int i = 0; i < KS / 2; ++i) {
+                        const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (k_first ^ (i * 16)));
+                        w[2 * i] = u32x2{x[0], x[1]};
+                        w[2 * i + 1] = u32x2{x[2], x[3]};
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) w[i] = *reinterpret_cast<const u32x2 *>(kb + j * 4 * D + quad * (D / 4) + i * 8);
+                }
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    const u32x4 a = widen8(w[i][0], w[i][1], 1.0f);
+#pragma unroll
+                    for (int t = PL - 1; t >= 0; --t)
+#pragma unroll
+                        for (int c = 0; c < CT; ++c) s[c][j] = mma(a, q16[c][t][i], s[c][j]);
+                }
             }
-            f32x4 acc[CT];
-#pragma unroll
-            for (int c = 0; c < CT; ++c) acc[c] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-                const u32x4 a = widen8(w[i][0], w[i][1]);
-#pragma unroll
-                for (int t2 = PL - 1; t2 >= 0; --t2)
-#pragma unroll
-                    for (int c = 0; c < CT; ++c) acc[c] = mma(a, qf[c][t2][i], acc[c]);
-            }
-#pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[c][4 * j + i] = acc[c][i];
         }
 
-        __builtin_amdgcn_sched_barrier(0);
-        // V's scale enters the weight through the exponent, but where that could leave the exponent's range
-        const bool fold = vb >= 67 && vb <= 187;
-        const float shift = fold ? (float)((int)vb - 127) : 0.0f;
-        const float unfold = fold ? e8m0(254 - vb) : 1.0f;
-        const bool plain = __builtin_amdgcn_ballot_w64(!fold) != 0;
         u32x4 pf[CT][PL][2];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
             if (!every) {
+                const int lo = in ? vis_lo[c] - tv : 16, hi = vis_hi[c] - tv;
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[c][i] = (in && tv + i >= vis_lo[c] && tv + i < vis_hi[c]) ? s[c][i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) s[c][i >> 2][i & 3] = i >= lo && i < hi ? s[c][i >> 2][i & 3] : -INFINITY;
             }
-            float top = s[c][0];
+            const float f = ks * qscale[c];
+            float top = s[c][0][0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[c][i]);
-            top = quads_max(top * ks);
+            for (int i = 1; i < 16; ++i) top = fmaxf(top, s[c][i >> 2][i & 3]);
+            top = quads_max(top * f);
             // the maximum moves only when it has grown by 2^8: weights stay within f32 and bf16 meanwhile
             const bool grow = top > m[c] + 8.0f || (m[c] == -INFINITY && top > -INFINITY);
             if (__builtin_amdgcn_ballot_w64(grow)) {
                 const float m2 = grow ? top : m[c];
                 const float alpha = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[c] - m2);
                 m[c] = m2;
-                sum[c] *= alpha;
+                total[c] *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[c][d] *= alpha;
             }
-            const float off = shift - (m[c] == -INFINITY ? 0.0f : m[c]);
-            float add = 0.0f;
+            const float off = m[c] == -INFINITY ? 0.0f : -m[c];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[c][i] = __builtin_amdgcn_exp2f(fmaf(s[c][i], ks, off));
-                add += s[c][i];
-            }
-            sum[c] = fmaf(add, unfold, sum[c]);
-            if (plain) {
-                const float vs = fold ? 1.0f : e8m0(vb);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[c][i] *= vs;
-            }
+            for (int i = 0; i < 16; ++i) s[c][i >> 2][i & 3] = __builtin_amdgcn_exp2f(fmaf(s[c][i >> 2][i & 3], f, off));
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = s[c][8 * u + 2 * i], y = s[c][8 * u + 2 * i + 1];
+                    const float x = s[c][2 * u + (i >> 1)][2 * (i & 1)], y = s[c][2 * u + (i >> 1)][2 * (i & 1) + 1];
                     if constexpr (BF) {
                         pf[c][0][u][i] = pair_near(x, y);
                     } else {
@@ -821,17 +884,23 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
                     }
                 }
         }
-        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();  // V is there
+        const char *vl = vbuf + v_at;
+        const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(vl + d * 1024);
-            const u32x4 a0 = widen8(v[0], v[1]), a1 = widen8(v[2], v[3]);
+        for (int d = 0; d <= DT; ++d) {
+            u32x4 a0 = one, a1 = one;
+            if (d < DT) {
+                a0 = *reinterpret_cast<const u32x4 *>(vl + d * 2048);
+                a1 = *reinterpret_cast<const u32x4 *>(vbuf + (v_at ^ 16) + d * 2048);
+            }
 #pragma unroll
             for (int t = PL - 1; t >= 0; --t)
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
-                    o[c][d] = mma(a0, pf[c][t][0], o[c][d]);
-                    o[c][d] = mma(a1, pf[c][t][1], o[c][d]);
+                    f32x4 &acc = d < DT ? o[c][d < DT ? d : 0] : total[c];
+                    acc = mma(a0, pf[c][t][0], acc);
+                    acc = mma(a1, pf[c][t][1], acc);
                 }
         }
         buf ^= 1;
@@ -850,28 +919,31 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
     }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-        sum[c] += __shfl_xor(sum[c], 16);
-        sum[c] += __shfl_xor(sum[c], 32);
+        const float sum = total[c][0];
         const int r = row0 + (wave * CT + c) * 16 + col;
         if (r >= rows) continue;
         const int h = head * group + r % group;
         if (splits == 1) {
-            const float inv = sum[c] == 0.0f ? 0.0f : 1.0f / sum[c];  // nothing seen: zero
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // nothing seen: zero
             const int64_t at = (start + r / group) * p.out_ld + (int64_t)h * D + quad * 4;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (BF) static_cast<__bf16 *>(p.out)[at + d * 16 + i] = (__bf16)(o[c][d][i] * inv);
-                    else static_cast<float *>(p.out)[at + d * 16 + i] = o[c][d][i] * inv;
+            for (int d = 0; d < DT; ++d) {
+                if constexpr (BF) {
+                    struct __attribute__((packed, aligned(2))) T4 { u32x2 v; };
+                    reinterpret_cast<T4 *>(static_cast<uint16_t *>(p.out) + at + d * 16)->v =
+                        u32x2{pair_near(o[c][d][0] * inv, o[c][d][1] * inv), pair_near(o[c][d][2] * inv, o[c][d][3] * inv)};
+                } else {
+                    struct __attribute__((packed, aligned(4))) T4 { f32x4 v; };
+                    reinterpret_cast<T4 *>(static_cast<float *>(p.out) + at + d * 16)->v = o[c][d] * inv;
                 }
+            }
         } else {
             const int64_t at = ((int64_t)split * rows_total + (int64_t)b * p.b.max_new + r / group) * p.q_heads + h;
 #pragma unroll
             for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(part.o + at * D + d * 16 + quad * 4) = o[c][d];
             if (quad == 0) {
                 part.ml[at * 2] = m[c];
-                part.ml[at * 2 + 1] = sum[c];
+                part.ml[at * 2 + 1] = sum;
             }
         }
     }
@@ -961,13 +1033,17 @@ hipError_t attend(const KvAttend &p, const KvPlan &pl, void *workspace, hipStrea
     part.ml = part.o + (size_t)pl.splits * rows_total * p.q_heads * p.c.dim;
     const dim3 rows_grid((unsigned)(pl.splits * row_tiles), (unsigned)p.c.heads, (unsigned)p.b.batch);
     const dim3 tiles_grid((unsigned)(pl.splits * row_tiles * p.c.heads), (unsigned)p.b.batch);
-#define DMC_DIM(N)                                                                                                        \
-    case N:                                                                                                               \
-        if (pl.kind == 0)                                                                                                 \
+    hipError_t e = hipSuccess;
+#define DMC_DIM(N)                                                                                                     \
+    case N:                                                                                                            \
+        if (pl.kind == 0) {                                                                                            \
             kv_rows_kernel<N, BF><<<rows_grid, dim3(256), 0, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total); \
-        else                                                                                                              \
-            kv_tiles_kernel<N, BF, kTiles<N, BF>>                                                                         \
-                <<<tiles_grid, dim3(256), 0, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total);              \
+        } else {                                                                                                       \
+            auto f = p.c.page >= kStep ? kv_tiles_kernel<N, BF, kTiles<N, BF>, true> : kv_tiles_kernel<N, BF, kTiles<N, BF>, false>; \
+            e = hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, KvTile<N>::LDS); \
+            if (e != hipSuccess) return e;                                                                             \
+            f<<<tiles_grid, dim3(256), KvTile<N>::LDS, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total); \
+        }                                                                                                              \
         break;
     switch (p.c.dim) {
         DMC_DIM(64)
@@ -976,7 +1052,7 @@ hipError_t attend(const KvAttend &p, const KvPlan &pl, void *workspace, hipStrea
         DMC_DIM(256)
     }
 #undef DMC_DIM
-    hipError_t e = hipGetLastError();
+    e = hipGetLastError();
     if (e == hipSuccess && pl.splits > 1) {
         kv_join_kernel<BF><<<dim3((unsigned)p.b.max_new, (unsigned)p.q_heads, (unsigned)p.b.batch), dim3(256), 0, stream>>>(
             p, part, pl.splits, pl.chunk, R, rows_total);

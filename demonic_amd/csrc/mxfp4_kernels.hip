@@ -484,39 +484,27 @@ __global__ __launch_bounds__(64 * WN * WM) void mx_tile_kernel(const MxTileArgs 
         for (int j = 0; j < CT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
     copy(g0, lds);
     copy(g0 + SK, lds + T::kStage);
-    int stage = 0;
-    for (int g = g0; g < g1; g += SK) {
-        // this stage has arrived (the next may be in flight) and the last one's reads are done
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kCopies) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        const int into = stage + 2 >= T::kDepth ? stage + 2 - T::kDepth : stage + 2;
-        copy(g + 2 * SK, lds + into * T::kStage);
-        const char *base = lds + stage * T::kStage;
+    auto group = [&](const char *gb) {
+        i32x8 a[RT];
+        int as[RT];
 #pragma unroll
-        for (int h = 0; h < SK; ++h) {
-            if (h && g + h >= g1) break;
-            const char *gb = base + h * T::kGroup;
-            i32x8 a[RT];
-            int as[RT];
+        for (int i = 0; i < RT; ++i) {
+            const u32x4 t = *reinterpret_cast<const u32x4 *>(gb + ((wn * RT + i) * 64 + lane) * 16);
+            a[i] = i32x8{(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
+            as[i] = *reinterpret_cast<const uint8_t *>(gb + T::kWq + T::kXq + ((wn * RT + i) * 16 + r) * 4 + quad);
+        }
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                const u32x4 t = *reinterpret_cast<const u32x4 *>(gb + ((wn * RT + i) * 64 + lane) * 16);
-                a[i] = i32x8{(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
-                as[i] = *reinterpret_cast<const uint8_t *>(gb + T::kWq + T::kXq + ((wn * RT + i) * 16 + r) * 4 + quad);
-            }
+        for (int j = 0; j < CT; ++j) {
+            if constexpr (PL == 1) {
+                const u32x4 t = *reinterpret_cast<const u32x4 *>(gb + T::kWq + ((wm * CT + j) * 64 + lane) * 16);
+                const i32x8 b = {(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
+                const int bs = *reinterpret_cast<const uint8_t *>(gb + T::kWq + T::kXq + T::kWs + ((wm * CT + j) * 16 + r) * 4 + quad);
 #pragma unroll
-            for (int j = 0; j < CT; ++j) {
-                if constexpr (PL == 1) {
-                    const u32x4 t = *reinterpret_cast<const u32x4 *>(gb + T::kWq + ((wm * CT + j) * 64 + lane) * 16);
-                    const i32x8 b = {(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
-                    const int bs = *reinterpret_cast<const uint8_t *>(gb + T::kWq + T::kXq + T::kWs + ((wm * CT + j) * 16 + r) * 4 + quad);
-#pragma unroll
-                    for (int i = 0; i < RT; ++i)
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 4, 0, as[i], 0, bs);
-                } else {
-                    const char *xb = gb + T::kWq + (wm * CT + j) * kUnit;
-                    const u32x2 sc = *reinterpret_cast<const u32x2 *>(xb + kUnitScales + lane * 8);
+                for (int i = 0; i < RT; ++i)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 4, 0, as[i], 0, bs);
+            } else {
+                const char *xb = gb + T::kWq + (wm * CT + j) * kUnit;
+                const u32x2 sc = *reinterpret_cast<const u32x2 *>(xb + kUnitScales + lane * 8);
 #define DMC_DIGIT(P, SEL, WORD)                                                                                       \
     {                                                                                                                 \
         const u32x4 t0 = *reinterpret_cast<const u32x4 *>(xb + P * 1536 + lane * 16);                                 \
@@ -524,17 +512,34 @@ __global__ __launch_bounds__(64 * WN * WM) void mx_tile_kernel(const MxTileArgs 
         const i32x8 b = {(int)t0[0], (int)t0[1], (int)t0[2], (int)t0[3], (int)t1[0], (int)t1[1], 0, 0};               \
         _Pragma("unroll") for (int i = 0; i < RT; ++i) acc[i][j] =                                                    \
             __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 2, 0, as[i], SEL, (int)sc[WORD]); \
-    }
-                    DMC_DIGIT(4, 0, 1)
-                    DMC_DIGIT(3, 3, 0)
-                    DMC_DIGIT(2, 2, 0)
-                    DMC_DIGIT(1, 1, 0)
-                    DMC_DIGIT(0, 0, 0)
+}
+                DMC_DIGIT(4, 0, 1)
+                DMC_DIGIT(3, 3, 0)
+                DMC_DIGIT(2, 2, 0)
+                DMC_DIGIT(1, 1, 0)
+                DMC_DIGIT(0, 0, 0)
 #undef DMC_DIGIT
-                }
             }
         }
+    };
+    int stage = 0, g = g0;
+    // this stage has arrived (the next may be in flight) and the last one's reads are done
+    auto arrive = [&]() {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kCopies) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    for (; g + SK <= g1; g += SK) {
+        arrive();
+        const int into = stage + 2 >= T::kDepth ? stage + 2 - T::kDepth : stage + 2;
+        copy(g + 2 * SK, lds + into * T::kStage);
+#pragma unroll
+        for (int h = 0; h < SK; ++h) group(lds + stage * T::kStage + h * T::kGroup);
         stage = stage + 1 == T::kDepth ? 0 : stage + 1;
+    }
+    if (SK > 1 && g < g1) {  // half a stage
+        arrive();
+        group(lds + stage * T::kStage);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives its workgroup's LDS
     float *y = p.y + (int64_t)slice * p.m * p.n;
@@ -605,10 +610,10 @@ hipError_t launch_mx_dequantize(const MxCast &p, hipStream_t stream) {
 
 // The tile shapes, by number: template arguments, and a launch of each.
 #define DMC_MX_SHAPES(X)                                            \
-    X(0, 1, 8, 4, 2, 2, 2) /* 256 x 128 */                          \
+    X(0, 1, 4, 4, 4, 2, 2) /* 256 x 128 */                          \
     X(1, 1, 2, 4, 4, 1, 2) /* 128 x 64 */                           \
     X(2, 1, 1, 1, 4, 1, 2) /* 64 x 16 */                            \
-    X(3, kDigits, 8, 2, 2, 2, 1) /* 256 x 64 */                     \
+    X(3, kDigits, 4, 2, 4, 2, 1) /* 256 x 64 */                     \
     X(4, kDigits, 2, 2, 4, 1, 1) /* 128 x 32 */                     \
     X(5, kDigits, 1, 1, 4, 1, 1) /* 64 x 16 */                      \
     X(6, kDigits, 4, 1, 4, 1, 1) /* 256 x 16 */
