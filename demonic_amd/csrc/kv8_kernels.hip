@@ -308,6 +308,13 @@ __device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i'
                                      (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
 }
 
+// A barrier for LDS alone: __syncthreads() would also wait for copies to LDS that are in flight.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ float quads_max(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
@@ -584,11 +591,18 @@ struct KvTile {
     static constexpr int RAW = kStep * D;                    // bytes of one side's codes
     static constexpr int PASSES = (kStep * KC + 255) / 256;  // pieces per thread and side
     static constexpr int LDS = 2 * 2 * RAW + 2 * RAW;        // two stages of codes, V in bf16
-    static __device__ __forceinline__ int k_slot(int t, int c) {
-        if (KC == 16) return c ^ ((t & 3) | ((t >> 2) & 12));
-        if (KC == 8) return c ^ (((t >> 1) & 1) | ((t >> 3) & 6));
-        if (KC == 4) return c ^ ((t >> 4) & 3);
-        return c;
+    // A 16-byte LDS read serves lanes 0-3, 12-15 and 20-27 at a time, then 4-11, 16-19 and 28-31, and so on: rows
+    // 0-3 and 12-15 of one quad with rows 4-11 of the next.  So a quad's n-th piece has place quad + 4 n, turned by a
+    // key that tells apart the rows of a 256-byte window and keeps neighbouring quads' rows apart too.
+    static __device__ __forceinline__ int k_key(int t) {
+        return KC == 16 ? (t & 3) | ((t >> 2) & 12) : KC == 8 ? ((t >> 1) & 1) | ((t >> 3) & 6) : KC == 4 ? -(t >> 4) & 3 : 0;
+    }
+    // The piece of a K row at place s (before the key), as its readers number them: bf16 rows read 32 bytes at
+    // 128 n + 32 quad, f32 rows D / 4 bytes at D / 4 quad.
+    static __device__ __forceinline__ int k_piece(bool bf, int s) {
+        if (KC == 6) return s;
+        if (!bf) return (s & 3) * (KC / 4) + (s >> 2);
+        return KC == 4 ? 2 * (s & 1) + (s >> 1) : 8 * (s >> 3) + 2 * (s & 3) + ((s >> 2) & 1);
     }
 };
 
@@ -702,7 +716,7 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
     for (int i = 0; i < T::PASSES; ++i) {
         const int at = i * 256 + threadIdx.x;
         kt[i] = at / T::KC;
-        ko[i] = kt[i] * D + T::k_slot(kt[i], at % T::KC) * 16;
+        ko[i] = kt[i] * D + T::k_piece(BF, (at % T::KC) ^ T::k_key(kt[i])) * 16;
         vo[i] = (at >> 2) * P + vc * 16;
     }
     constexpr int IDS = UP ? 1 : T::PASSES;
@@ -747,9 +761,12 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
     }
     // this lane's K pieces (token rows 4 j on) and V pieces
     const int k_tok = 16 * (col >> 2) + (col & 3);
-    const int k_piece = BF ? (D == 64 ? 2 * (quad & 1) : D == 96 ? min(2 * quad, 4) : 2 * quad) : (KS % 2 == 0 ? quad * (KS / 2) : 0);
-    const int k_at = k_tok * D, k_first = T::k_slot(k_tok, k_piece) * 16;
-    const int v_at = col * 128 + (((2 * quad) ^ ((col >> 1) & 7)) * 16);
+    // the dim of a wave's 16 that this thread widens: 8 lanes write two dims 8 apart, whose places differ
+    const int v_dim = ((lane >> 2) & 1) * 8 + (lane >> 3);
+    const int k_at = k_tok * D;
+    const int k_first = T::KC == 6 ? min(quad, 2) * 32 : ((BF && D == 64 ? quad & 1 : quad) ^ T::k_key(k_tok)) * 16;
+    constexpr int K_NEXT = D == 64 ? 32 : 64;  // from a piece's place to the next one's, by exclusive or
+    const int v_at = col * 128 + ((quad ^ ((col >> 1) & 7)) * 16);
     int buf = 0;
     if (threadIdx.x == 0) nans = 0;
     if (from < to) {
@@ -781,11 +798,13 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
 #pragma unroll
         for (int i = 0; i < T::PASSES; ++i) {
             if (!live(i)) break;
-            const int at = i * 256 + threadIdx.x, dim = at >> 2;
-            u32x4 v = *reinterpret_cast<const u32x4 *>(raw + T::RAW + at * 16);
+            const int dim = (i * 4 + wave) * 16 + v_dim;
+            u32x4 v = *reinterpret_cast<const u32x4 *>(raw + T::RAW + (dim * 4 + vc) * 16);
             if (!whole || !v_in) {
                 // codes that no row sees read as zero, and so do NaN codes, for now (nan_dims)
-                const int tt = t0 + 16 * vc, hi = v_in ? see_hi : 0;
+                int tt = t0 + 16 * vc;
+                asm volatile("" : "+v"(tt));  // rare: the masks are not to be formed ahead of the branch
+                const int hi = v_in ? see_hi : 0;
                 uint32_t bad = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -797,8 +816,8 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
             }
             char *w = vbuf + dim * 128;
             const int key = (dim >> 1) & 7;
-            *reinterpret_cast<u32x4 *>(w + ((2 * vc) ^ key) * 16) = widen8(v[0], v[1], vs);
-            *reinterpret_cast<u32x4 *>(w + ((2 * vc + 1) ^ key) * 16) = widen8(v[2], v[3], vs);
+            *reinterpret_cast<u32x4 *>(w + (vc ^ key) * 16) = widen8(v[0], v[1], vs);
+            *reinterpret_cast<u32x4 *>(w + ((vc + 4) ^ key) * 16) = widen8(v[2], v[3], vs);
         }
 
         // scores
@@ -811,8 +830,8 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
             if constexpr (BF) {
 #pragma unroll
                 for (int h = 0; h < QC; ++h) {
-                    u32x4 lo = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + ((k_first ^ (h * 128)))),
-                          hi = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (KvTile<D>::KC == 6 ? k_first + 16 : k_first ^ (h * 128 + 16)));
+                    u32x4 lo = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (k_first ^ (2 * h * K_NEXT))),
+                          hi = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (T::KC == 6 ? k_first + 16 : k_first ^ ((2 * h + 1) * K_NEXT)));
                     if (D == 96 && quad == 3) lo = hi = u32x4{0, 0, 0, 0};
                     const i32x8 a = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 #pragma unroll
@@ -826,7 +845,7 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
                 if constexpr (KS % 2 == 0) {
 #pragma unroll
                     for (int i = 0; i < KS / 2; ++i) {
-                        const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (k_first ^ (i * 16)));
+                        const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + j * 4 * D + (k_first ^ (i * K_NEXT)));
                         w[2 * i] = u32x2{x[0], x[1]};
                         w[2 * i + 1] = u32x2{x[2], x[3]};
                     }
@@ -884,7 +903,7 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
                     }
                 }
         }
-        __syncthreads();  // V is there
+        lds_barrier();  // V is there; the next step's codes stay in flight
         const char *vl = vbuf + v_at;
         const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
@@ -892,7 +911,7 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
             u32x4 a0 = one, a1 = one;
             if (d < DT) {
                 a0 = *reinterpret_cast<const u32x4 *>(vl + d * 2048);
-                a1 = *reinterpret_cast<const u32x4 *>(vbuf + (v_at ^ 16) + d * 2048);
+                a1 = *reinterpret_cast<const u32x4 *>(vbuf + (v_at ^ 64) + d * 2048);
             }
 #pragma unroll
             for (int t = PL - 1; t >= 0; --t)
