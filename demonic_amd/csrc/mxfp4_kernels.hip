@@ -391,6 +391,7 @@ struct MxTileArgs {
     int m, k, n, groups, rtiles;
     int ntn, ntm;              // tiles along n and m
     int slices, per;           // slices of k, groups of each
+    bool wide_scales;          // rows of scales are 16-byte aligned, slices too
 };
 
 __device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i's 16 bytes to l + 16 i
@@ -403,26 +404,33 @@ __device__ __forceinline__ void lds_copy4(const void *g, char *l) {  // lane i's
 }
 
 // Tiles of TN weight rows x TM activation rows; WN x WM waves of RT x CT MFMA tiles.  Both sides go to LDS without
-// passing through registers, SK groups of 128 k per stage, three stages deep, in the order that a lane reads its
-// operands in (16 rows x 4 blocks: lane 16 q + r's 16 bytes at 16 (16 q + r)), so that reads meet no bank twice.
+// passing through registers, SK groups of 128 k per stage, three stages deep.
+//
+// What bounds this is first how loads are asked for: a lane that reads 16 bytes of another row than its neighbour
+// costs the L1 an access of its own, so the lanes of a copy take whole row pieces (8 lanes a 128-byte line at SK = 2,
+// 4 half a line at SK = 1), and a row's scales come for four groups at a time (16 bytes).  An operand read takes
+// 16 rows' pieces at once; the piece p of row r lies at place p ^ (r / 2), so that no two meet a bank.
 template <int PL, int RT, int CT, int WN, int WM, int SK>
 struct MxTile {
     static constexpr int kWaves = WN * WM, TN = WN * RT * 16, TM = WM * CT * 16;
-    static constexpr int kWq = TN * 64, kWs = (TN + 63) / 64 * 256;
-    static constexpr int kXq = PL == 1 ? TM * 64 : TM / 16 * kUnit, kXs = PL == 1 ? (TM + 63) / 64 * 256 : 0;
-    static constexpr int kGroup = kWq + kXq + kWs + kXs;  // LDS bytes of a group of k
-    static constexpr int kStage = SK * kGroup;
-    static constexpr int kBig = (kWq + kXq) / 1024, kSmall = (kWs + kXs) / 256;  // copies of a group
-    static constexpr int kBigEach = (kBig * SK + kWaves - 1) / kWaves, kSmallEach = (kSmall * SK + kWaves - 1) / kWaves;
-    static constexpr int kCopies = kBigEach + kSmallEach;  // of a wave per stage
+    static constexpr int kPitch = 64 * SK;  // bytes of a row in a stage
+    static constexpr int kWq = TN * kPitch, kXq = PL == 1 ? TM * kPitch : SK * (TM / 16) * kUnit;
+    static constexpr int kStage = kWq + kXq;
+    static constexpr int kCopies = (kStage / 1024 + kWaves - 1) / kWaves;  // of a wave per stage, 1 KB each
     static constexpr int kDepth = 3;
-    static_assert(kDepth * kStage <= 160 * 1024 && kCopies < 32, "");
+    static constexpr int kScaleRows = (TN + 63) / 64 * 64 + (PL == 1 ? (TM + 63) / 64 * 64 : 0);
+    static constexpr int kScales = kScaleRows * 16;  // bytes of four groups' scales
+    static constexpr int kScaleCopies = (kScaleRows / 64 + kWaves - 1) / kWaves;
+    static constexpr int kLds = kDepth * kStage + 2 * kScales;
+    static_assert(kLds <= 160 * 1024 && kCopies < 32 && kStage % 1024 == 0, "");
+    static __device__ __forceinline__ int key(int row) { return (row >> 1) & (4 * SK - 1); }
 };
 
 template <int PL, int RT, int CT, int WN, int WM, int SK>
 __global__ __launch_bounds__(64 * WN * WM) void mx_tile_kernel(const MxTileArgs p) {
     using T = MxTile<PL, RT, CT, WN, WM, SK>;
     extern __shared__ char lds[];
+    char *const scales = lds + T::kDepth * T::kStage;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r = lane & 15, quad = lane >> 4;
     const int wn = wave % WN, wm = wave / WN;
@@ -439,42 +447,58 @@ __global__ __launch_bounds__(64 * WN * WM) void mx_tile_kernel(const MxTileArgs 
     const int64_t qrow = (int64_t)p.groups * 64, srow = (int64_t)p.groups * 4;
 
     // this wave's copies of a stage (past the last one: the last one again)
-    const uint8_t *big[T::kBigEach], *small_[T::kSmallEach];
-    int big_lds[T::kBigEach], small_lds[T::kSmallEach], big_g[T::kBigEach], small_g[T::kSmallEach];
-    bool big_x[T::kBigEach];
+    constexpr int kRows = 16 / SK;  // rows of a copy
+    const uint8_t *src[T::kCopies];
+    int piece[T::kCopies];          // row copies: the lane's piece; digits: the unit's group
+    bool digits[T::kCopies];
 #pragma unroll
-    for (int i = 0; i < T::kBigEach; ++i) {
-        const int c = min(wave + i * T::kWaves, T::kBig * SK - 1), half = c / T::kBig, at = c - half * T::kBig;
-        big_g[i] = half;
-        big_lds[i] = half * T::kGroup + at * 1024;
-        big_x[i] = at >= T::kWq / 1024;
-        if (!big_x[i]) {
-            const int64_t row = min(n0 + at * 16 + r, (int64_t)p.n - 1);
-            big[i] = p.wq + row * qrow + quad * 16;
-        } else if (PL == 1) {
-            const int64_t row = min(m0 + (at - T::kWq / 1024) * 16 + r, p.m - 1);
-            big[i] = p.xq + row * qrow + quad * 16;
+    for (int i = 0; i < T::kCopies; ++i) {
+        const int c = min(wave + i * T::kWaves, T::kStage / 1024 - 1);
+        digits[i] = PL > 1 && c >= T::kWq / 1024;
+        if (digits[i]) {
+            const int x = c - T::kWq / 1024, unit = x >> 3, tile = min((m0 >> 4) + unit % (T::TM / 16), p.rtiles - 1);
+            piece[i] = unit / (T::TM / 16);
+            src[i] = p.xq + (int64_t)tile * kUnit + (x & 7) * 1024 + lane * 16;
         } else {
-            const int xt = at - T::kWq / 1024, tile = min((m0 >> 4) + (xt >> 3), p.rtiles - 1);
-            big[i] = p.xq + (int64_t)tile * kUnit + (xt & 7) * 1024 + lane * 16;
+            const bool x = c >= T::kWq / 1024;
+            const int row = (c - (x ? T::kWq / 1024 : 0)) * kRows + lane / (4 * SK);
+            piece[i] = (lane & (4 * SK - 1)) ^ T::key(row);
+            src[i] = x ? p.xq + min((int64_t)m0 + row, (int64_t)p.m - 1) * qrow : p.wq + min(n0 + row, (int64_t)p.n - 1) * qrow;
         }
-    }
-#pragma unroll
-    for (int i = 0; i < T::kSmallEach; ++i) {
-        const int c = min(wave + i * T::kWaves, T::kSmall * SK - 1), half = c / T::kSmall, at = c - half * T::kSmall;
-        small_g[i] = half;
-        small_lds[i] = half * T::kGroup + T::kWq + T::kXq + at * 256;
-        if (at < T::kWs / 256) small_[i] = p.ws + min(n0 + at * 64 + lane, (int64_t)p.n - 1) * srow;
-        else small_[i] = p.xs + (int64_t)min(m0 + (at - T::kWs / 256) * 64 + lane, p.m - 1) * srow;
     }
     auto copy = [&](int g, char *to) {  // groups past the slice's end: its last one
 #pragma unroll
-        for (int i = 0; i < T::kBigEach; ++i) {
-            const int64_t at = min(g + big_g[i], g1 - 1);
-            lds_copy16(big[i] + (PL > 1 && big_x[i] ? at * p.rtiles * kUnit : at * 64), to + big_lds[i]);
+        for (int i = 0; i < T::kCopies; ++i) {
+            const int c = min(wave + i * T::kWaves, T::kStage / 1024 - 1);
+            if (digits[i]) {
+                lds_copy16(src[i] + (int64_t)min(g + piece[i], g1 - 1) * p.rtiles * kUnit, to + c * 1024);
+            } else {
+                const int at = min(g * 64 + piece[i] * 16, (g1 - 1) * 64 + (piece[i] & 3) * 16);
+                lds_copy16(src[i] + at, to + c * 1024);
+            }
         }
+    };
+    // Scales of four groups: 16 bytes a row, or (rows of scales that are not 16-byte aligned) four times 4.
+    const uint8_t *ssrc[T::kScaleCopies];
 #pragma unroll
-        for (int i = 0; i < T::kSmallEach; ++i) lds_copy4(small_[i] + (int64_t)min(g + small_g[i], g1 - 1) * 4, to + small_lds[i]);
+    for (int i = 0; i < T::kScaleCopies; ++i) {
+        const int row = min(wave + i * T::kWaves, T::kScaleRows / 64 - 1) * 64 + lane;
+        constexpr int kN = (T::TN + 63) / 64 * 64;
+        ssrc[i] = row < kN ? p.ws + min(n0 + row, (int64_t)p.n - 1) * srow
+                           : p.xs + min((int64_t)m0 + row - kN, (int64_t)p.m - 1) * srow;
+    }
+    const int s_row = p.wide_scales ? 16 : 4, s_group = p.wide_scales ? 4 : 4 * T::kScaleRows;
+    auto copy_scales = [&](int g, char *to) {
+#pragma unroll
+        for (int i = 0; i < T::kScaleCopies; ++i) {
+            const int c = min(wave + i * T::kWaves, T::kScaleRows / 64 - 1);
+            if (p.wide_scales) {
+                lds_copy16(ssrc[i] + min(g, p.groups - 4) * 4, to + c * 1024);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) lds_copy4(ssrc[i] + min(g + h, g1 - 1) * 4, to + h * 4 * T::kScaleRows + c * 256);
+            }
+        }
     };
 
     f32x4 acc[RT][CT];
@@ -482,37 +506,42 @@ __global__ __launch_bounds__(64 * WN * WM) void mx_tile_kernel(const MxTileArgs 
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int j = 0; j < CT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    copy_scales(g0, scales);
     copy(g0, lds);
     copy(g0 + SK, lds + T::kStage);
-    auto group = [&](const char *gb) {
+    // a lane's operands: row r of a 16-row tile (16 rows keep the key's period), piece 4 h + quad
+    const int w_at = (wn * RT * 16 + r) * T::kPitch, x_at = T::kWq + (wm * CT * 16 + r) * T::kPitch;
+    const int ws_at = (wn * RT * 16 + r) * s_row + quad, xs_at = ((T::TN + 63) / 64 * 64 + wm * CT * 16 + r) * s_row + quad;
+    auto group = [&](const char *base, const char *sc, int h) {
+        const int place = ((4 * h + quad) ^ T::key(r)) * 16;
         i32x8 a[RT];
         int as[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            const u32x4 t = *reinterpret_cast<const u32x4 *>(gb + ((wn * RT + i) * 64 + lane) * 16);
+            const u32x4 t = *reinterpret_cast<const u32x4 *>(base + w_at + i * 16 * T::kPitch + place);
             a[i] = i32x8{(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
-            as[i] = *reinterpret_cast<const uint8_t *>(gb + T::kWq + T::kXq + ((wn * RT + i) * 16 + r) * 4 + quad);
+            as[i] = *reinterpret_cast<const uint8_t *>(sc + ws_at + i * 16 * s_row);
         }
 #pragma unroll
         for (int j = 0; j < CT; ++j) {
             if constexpr (PL == 1) {
-                const u32x4 t = *reinterpret_cast<const u32x4 *>(gb + T::kWq + ((wm * CT + j) * 64 + lane) * 16);
+                const u32x4 t = *reinterpret_cast<const u32x4 *>(base + x_at + j * 16 * T::kPitch + place);
                 const i32x8 b = {(int)t[0], (int)t[1], (int)t[2], (int)t[3], 0, 0, 0, 0};
-                const int bs = *reinterpret_cast<const uint8_t *>(gb + T::kWq + T::kXq + T::kWs + ((wm * CT + j) * 16 + r) * 4 + quad);
+                const int bs = *reinterpret_cast<const uint8_t *>(sc + xs_at + j * 16 * s_row);
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
                     acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 4, 0, as[i], 0, bs);
             } else {
-                const char *xb = gb + T::kWq + (wm * CT + j) * kUnit;
-                const u32x2 sc = *reinterpret_cast<const u32x2 *>(xb + kUnitScales + lane * 8);
+                const char *xb = base + T::kWq + (h * (T::TM / 16) + wm * CT + j) * kUnit;
+                const u32x2 xs = *reinterpret_cast<const u32x2 *>(xb + kUnitScales + lane * 8);
 #define DMC_DIGIT(P, SEL, WORD)                                                                                       \
     {                                                                                                                 \
         const u32x4 t0 = *reinterpret_cast<const u32x4 *>(xb + P * 1536 + lane * 16);                                 \
         const u32x2 t1 = *reinterpret_cast<const u32x2 *>(xb + P * 1536 + 1024 + lane * 8);                           \
         const i32x8 b = {(int)t0[0], (int)t0[1], (int)t0[2], (int)t0[3], (int)t1[0], (int)t1[1], 0, 0};               \
         _Pragma("unroll") for (int i = 0; i < RT; ++i) acc[i][j] =                                                    \
-            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 2, 0, as[i], SEL, (int)sc[WORD]); \
-}
+            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b, acc[i][j], 4, 2, 0, as[i], SEL, (int)xs[WORD]); \
+    }
                 DMC_DIGIT(4, 0, 1)
                 DMC_DIGIT(3, 3, 0)
                 DMC_DIGIT(2, 2, 0)
@@ -523,7 +552,8 @@ __global__ __launch_bounds__(64 * WN * WM) void mx_tile_kernel(const MxTileArgs 
         }
     };
     int stage = 0, g = g0;
-    // this stage has arrived (the next may be in flight) and the last one's reads are done
+    // This stage has arrived (the next may be in flight, but not the scales asked for before it) and the last one's
+    // reads are done.
     auto arrive = [&]() {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kCopies) : "memory");
         __builtin_amdgcn_s_barrier();
@@ -531,15 +561,17 @@ __global__ __launch_bounds__(64 * WN * WM) void mx_tile_kernel(const MxTileArgs 
     };
     for (; g + SK <= g1; g += SK) {
         arrive();
-        const int into = stage + 2 >= T::kDepth ? stage + 2 - T::kDepth : stage + 2;
+        const int at = g - g0, into = stage + 2 >= T::kDepth ? stage + 2 - T::kDepth : stage + 2;
+        char *const sc = scales + ((at >> 2) & 1) * T::kScales;
+        if ((at & 3) == 0) copy_scales(g + 4, scales + (((at >> 2) & 1) ^ 1) * T::kScales);
         copy(g + 2 * SK, lds + into * T::kStage);
 #pragma unroll
-        for (int h = 0; h < SK; ++h) group(lds + stage * T::kStage + h * T::kGroup);
+        for (int h = 0; h < SK; ++h) group(lds + stage * T::kStage, sc + ((at & 3) + h) * s_group, h);
         stage = stage + 1 == T::kDepth ? 0 : stage + 1;
     }
     if (SK > 1 && g < g1) {  // half a stage
         arrive();
-        group(lds + stage * T::kStage);
+        group(lds + stage * T::kStage, scales + (((g - g0) >> 2) & 1) * T::kScales + ((g - g0) & 3) * s_group, 0);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy outlives its workgroup's LDS
     float *y = p.y + (int64_t)slice * p.m * p.n;
@@ -614,9 +646,9 @@ hipError_t launch_mx_dequantize(const MxCast &p, hipStream_t stream) {
     X(1, 1, 2, 4, 4, 1, 2) /* 128 x 64 */                           \
     X(2, 1, 1, 1, 4, 1, 2) /* 64 x 16 */                            \
     X(3, kDigits, 4, 2, 4, 2, 1) /* 256 x 64 */                     \
-    X(4, kDigits, 2, 2, 4, 1, 1) /* 128 x 32 */                     \
-    X(5, kDigits, 1, 1, 4, 1, 1) /* 64 x 16 */                      \
-    X(6, kDigits, 4, 1, 4, 1, 1) /* 256 x 16 */
+    X(4, kDigits, 2, 2, 4, 1, 2) /* 128 x 32 */                     \
+    X(5, kDigits, 1, 1, 4, 1, 2) /* 64 x 16 */                      \
+    X(6, kDigits, 4, 1, 4, 1, 2) /* 256 x 16 */
 
 namespace {
 struct Shape { int tn, tm; };
@@ -632,7 +664,7 @@ hipError_t launch_shape(int shape, const MxTileArgs &a, hipStream_t stream) {
 #define X(ID, PL, RT, CT, WN, WM, SK)                                                                                   \
     case ID: {                                                                                                        \
         auto f = mx_tile_kernel<PL, RT, CT, WN, WM, SK>;                                                               \
-        constexpr int lds = MxTile<PL, RT, CT, WN, WM, SK>::kDepth * MxTile<PL, RT, CT, WN, WM, SK>::kStage;           \
+        constexpr int lds = MxTile<PL, RT, CT, WN, WM, SK>::kLds;                                                      \
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(f),                                    \
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);                     \
         if (e != hipSuccess) return e;                                                                                 \
@@ -668,7 +700,7 @@ MxPlan plan_mx(const MxProblem &p, int num_cus) {
         const int64_t most = std::max<int64_t>(1, groups / 8);
         pl.slices = (int)std::min<int64_t>(most, num_cus / pl.grid_x);
     }
-    pl.per = (int)((groups + pl.slices - 1) / pl.slices);
+    pl.per = (int)((groups + pl.slices - 1) / pl.slices + 3) / 4 * 4;
     pl.slices = (int)((groups + pl.per - 1) / pl.per);
     pl.workspace_bytes = p.x ? digits_bytes(p.m, p.k) : 0;
     if (pl.slices > 1) pl.workspace_bytes += (size_t)pl.slices * p.m * p.n * 4;
@@ -703,6 +735,7 @@ hipError_t launch_mx(const MxProblem &p, const MxPlan &pl, void *workspace, hipS
     a.ntm = div_up(p.m, kShapes[pl.shape].tm);
     a.slices = pl.slices;
     a.per = pl.per;
+    a.wide_scales = a.groups % 4 == 0 && (reinterpret_cast<uintptr_t>(p.ws) | reinterpret_cast<uintptr_t>(p.xs)) % 16 == 0;
     char *w = static_cast<char *>(workspace);
     if (p.x) {
         mx_split_kernel<<<dim3((unsigned)((int64_t)a.groups * a.rtiles)), dim3(256), 0, stream>>>(p.x, w, a.m, a.k, a.rtiles);
