@@ -308,6 +308,21 @@ __device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i'
                                      (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
 }
 
+// Bits lo .. hi - 1 of 16, and a score where its bit is set, else -inf (by bits: 16 lane masks would not fit the
+// scalar registers).
+__device__ __forceinline__ uint32_t seen16(int lo, int hi) {
+    return ((1u << min(max(hi, 0), 16)) - 1u) & ~((1u << min(max(lo, 0), 16)) - 1u);
+}
+__device__ __forceinline__ float keep_seen(float s, uint32_t bits, int i) {
+    const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)bits, i, 1);
+    return __uint_as_float((__float_as_uint(s) & m) | (0xff800000u & ~m));
+}
+
+// A dword, the same for all lanes, that no kernel writes meanwhile: through the scalar cache.
+__device__ __forceinline__ uint32_t scalar_load(const void *p) {
+    return *reinterpret_cast<const __attribute__((address_space(4))) uint32_t *>(reinterpret_cast<uintptr_t>(p));
+}
+
 // A barrier for LDS alone: __syncthreads() would also wait for copies to LDS that are in flight.
 __device__ __forceinline__ void lds_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -327,18 +342,35 @@ struct KvPart {
     float *ml; // [splits][rows][2]
 };
 
-// Workgroups (column tile, token split), heads, sequences; 4 waves take steps of 64 tokens in turn.  A step's V is
-// on its way to registers while its scores are formed, the next step's K from then on (into the registers
-// that held this one's), so that each wave has 8 to 16 KB in flight without a second set of registers.
-template <int D, bool BF>
+// Workgroups (column tile, token split), heads, sequences; NW waves take steps of 64 tokens in turn.  A wave's codes
+// go to LDS of its own without passing through registers, by copies whose lanes take whole rows (lanes that read 16
+// bytes of different rows each cost the L1 an access): the next step's K once this one's scores are formed, its V
+// once this one's is read, so that one place each is enough and 2 workgroups fit a CU.  Only the wave itself waits.
+// 16-byte pieces lie turned by a key of their row, so that an operand read meets no bank twice.
+// UP: pages hold 64 tokens or more, so that a step lies in one.
+template <int D>
+struct KvRows {
+    static constexpr int NW = 4;
+    static constexpr int RAW = kStep * D;                   // bytes of one side's codes
+    static constexpr int KC = D / 16, PASSES = RAW / 1024;  // pieces of a K row; copies of a side
+    static constexpr int LDS = NW * 2 * RAW;
+    static __device__ __forceinline__ int k_key(int t) {  // rows 4 j + 16 (r / 4) + r % 4 are read together, r = 0 .. 15
+        return KC == 16 ? (t & 3) | ((t >> 2) & 12) : KC == 8 ? ((t >> 1) & 1) | ((t >> 3) & 6) : KC == 4 ? -(t >> 4) & 3 : 0;
+    }
+};
+
+template <int D, bool BF, bool UP>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const KvAttend p, const KvPart part, int splits, int chunk,
-                                                      int row_tiles, int64_t rows_total) {
+                                                                        int row_tiles, int64_t rows_total) {
+    using T = KvRows<D>;
+    constexpr int NW = T::NW, NT = 64 * NW;
     constexpr int R = BF ? 16 : 4;      // query rows per column tile
     constexpr int KS = D / 32;          // MFMA steps over dims
     constexpr int DT = D / 16;          // tiles of dims
     constexpr bool WIDE = KS % 2 == 0;  // K rows in 16-byte pieces (piece i of quad q: dims 64 i + 16 q on), else in 8
     constexpr int KP = WIDE ? KS / 2 : KS;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
     const int split = blockIdx.x / row_tiles, tile = blockIdx.x - split * row_tiles;
     const int head = blockIdx.y, b = blockIdx.z;
@@ -367,28 +399,69 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
     const int32_t *table = p.b.table + (int64_t)b * p.b.width;
     const float scale = p.scale * kLog2e;
     const int64_t page_bytes = (int64_t)P * D;
-    auto page_of = [&](int t) -> int {  // no branch: past the table, its last entry is read and not taken
-        const int id = table[min(t, most - 1) >> lgp];
-        return t < most && (uint32_t)id < (uint32_t)p.c.pages ? id : -1;
+    // A table entry as it is, and what it names for token t.  Through vector registers a use waits for every copy asked
+    // for before too, so that entries and scales are asked for a step ahead; where all lanes want the same one, it
+    // comes through the scalar cache, which counts apart.
+    auto entry = [&](int t) -> int {
+        const int32_t *at = table + (min(t, most - 1) >> lgp);
+        return UP ? (int)scalar_load(at) : *at;
     };
-    auto safe = [&](int id) -> int64_t { return max(id, 0); };
-    u32x4 kw[WIDE ? 4 * KP : 1];
-    u32x2 k8[WIDE ? 1 : 4 * KP];
-    // pk: the page of the 16 tokens that this lane's K rows (r / 4) lie in, pv: of this lane's own tokens
-    auto load_k = [&](int t0, int pk) {
-        const uint8_t *kp = p.c.k + (safe(pk) * p.c.heads + head) * page_bytes + (((t0 + 16 * (col >> 2)) & (P - 1)) + (col & 3)) * D;
+    auto page_at = [&](int id, int t) -> int { return t < most && (uint32_t)id < (uint32_t)p.c.pages ? id : -1; };
+    auto scale_of = [&](const uint8_t *scales, int page) -> uint32_t {
+        const uint8_t *at = scales + max(page, 0) * (int64_t)p.c.heads + head;
+        if constexpr (UP) {  // the dword that holds the byte
+            const uint64_t a = reinterpret_cast<uint64_t>(at);
+            return (scalar_load(reinterpret_cast<const void *>(a & ~3ull)) >> (8 * (a & 3))) & 255u;
+        }
+        return *at;
+    };
+    const uint8_t *const kh = p.c.k + head * page_bytes, *const vh = p.c.v + head * page_bytes;
+    const int64_t stride = page_bytes * p.c.heads;
+    char *const mine = lds + wave * (2 * T::RAW);
+    // this lane's place in a copy: V dim v_dim (+ 16 per copy), its 16 tokens vc; K by row
+    const int v_dim = lane >> 2, vc = (lane & 3) ^ ((v_dim >> 1) & 3), vo = v_dim * P + vc * 16;
+    int kid[UP ? 1 : 4], vid = 0;
+    auto ids = [&](int t0) {
+        if constexpr (UP) {
+            kid[0] = entry(t0);  // one register for all uses: a copy would wait for the load
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j) kid[j] = entry(t0 + 16 * j);
+            vid = entry(t0 + 16 * vc);
+        }
+    };
+    auto fetch_k = [&](int t0) {
+        const int in = t0 & (P - 1);
 #pragma unroll
-            for (int i = 0; i < KP; ++i) {
-                if constexpr (WIDE) kw[j * KP + i] = *reinterpret_cast<const u32x4 *>(kp + j * 4 * D + i * 64 + quad * 16);
-                else k8[j * KP + i] = *reinterpret_cast<const u32x2 *>(kp + j * 4 * D + i * 32 + quad * 8);
+        for (int i = 0; i < T::PASSES; ++i) {
+            const int at = i * 64 + lane, t = at / T::KC, off = t * D + ((at % T::KC) ^ T::k_key(t)) * 16;
+            if constexpr (UP) {
+                lds_copy16(kh + max(page_at(kid[0], t0), 0) * stride + in * D + off, mine + i * 1024);
+            } else {
+                const int g = t >> 4;
+                const int id = D != 96 ? kid[(i * 64 / T::KC) >> 4] : g == 0 ? kid[0] : g == 1 ? kid[1] : g == 2 ? kid[2] : kid[3];
+                lds_copy16(kh + max(page_at(id, t0 + 16 * g), 0) * stride + (((t0 + 16 * g) & (P - 1)) - 16 * g) * D + off, mine + i * 1024);
             }
+        }
     };
-    const int first = from + wave * kStep, tko = 16 * (col >> 2), tvo = 16 * quad;
-    int pv = page_of(first + tvo), pk = page_of(first + 4 * kStep + tko), pv_next = page_of(first + 4 * kStep + tvo);
-    load_k(first, page_of(first + tko));
-    uint32_t ksb = p.c.ks[safe(pv) * p.c.heads + head], vsb = p.c.vs[safe(pv) * p.c.heads + head];
+    auto fetch_v = [&](int t0, int id) {
+        const uint8_t *v = vh + max(page_at(id, UP ? t0 : t0 + 16 * vc), 0) * stride + (UP ? t0 & (P - 1) : ((t0 + 16 * vc) & (P - 1)) - 16 * vc) + vo;
+#pragma unroll
+        for (int i = 0; i < T::PASSES; ++i) lds_copy16(v + i * 16 * P, mine + T::RAW + i * 1024);
+    };
+    const int first = from + wave * kStep, tvo = 16 * quad;
+    int own = -1, own_next = -1;
+    float ks_next = 0.0f, vs_next = 1.0f;
+    if (first < to) {  // a step ahead: codes, this lane's own 16 tokens' page and scales, and the pages of the step after
+        ids(first);
+        own = UP ? page_at(kid[0], first) : page_at(entry(first + tvo), first + tvo);
+        ks_next = e8m0(scale_of(p.c.ks, own)) * scale;
+        vs_next = own >= 0 ? e8m0(scale_of(p.c.vs, own)) : 1.0f;
+        fetch_k(first);
+        fetch_v(first, UP ? kid[0] : vid);
+        ids(first + NW * kStep);
+        if (!UP) own_next = entry(first + NW * kStep + tvo);
+    }
 
     u32x4 qf[KS];
 #pragma unroll
@@ -405,20 +478,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
         }
     }
 
+    // q and the first scales are waited for here, not in the loop, where that would be a wait for its copies
+#pragma unroll
+    for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
+    if (!UP) asm volatile("" : "+v"(ks_next), "+v"(vs_next));
+
     f32x4 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, sum = 0.0f;
     uint32_t nans = 0;
 
-    for (int t0 = first; t0 < to; t0 += 4 * kStep) {
+    // where this lane's operands lie: K rows 4 j on, pieces by 64 bytes; V dims 16 d on
+    const int k_tok = 16 * (col >> 2) + (col & 3);
+    const int k_at = k_tok * D + (WIDE ? (quad ^ T::k_key(k_tok)) * 16 : quad * 8);
+    const int v_at = T::RAW + col * 64 + (quad ^ ((col >> 1) & 3)) * 16;
+    for (int t0 = first; t0 < to; t0 += NW * kStep) {
+        // this step's K is there; its V, asked for last, may be on its way
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::PASSES) : "memory");
+        const char *const raw = mine;
         const int tv = t0 + tvo;
-        const bool in = pv >= 0;
-        u32x4 vw[DT];
-        const uint8_t *vp = p.c.v + (safe(pv) * p.c.heads + head) * page_bytes + col * P + (tv & (P - 1));
-#pragma unroll
-        for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4 *>(vp + d * 16 * P);
-        const float ks = e8m0(ksb) * scale, vs = in ? e8m0(vsb) : 1.0f;  // an absent page's byte may be any
+        const bool in = own >= 0;
+        const float ks = ks_next, vs = vs_next;
+        const int vid_next = UP ? kid[0] : vid;
         float s[16];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -426,24 +508,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
                 if constexpr (WIDE) {
-                    const u32x4 w = kw[j * KP + i];
+                    const u32x4 w = *reinterpret_cast<const u32x4 *>(raw + (k_at ^ (i * 64)) + j * 4 * D);
                     c = mma(widen8(w[0], w[1], 1.0f), qf[2 * i], c);
                     c = mma(widen8(w[2], w[3], 1.0f), qf[2 * i + 1], c);
                 } else {
-                    const u32x2 w = k8[j * KP + i];
+                    const u32x2 w = *reinterpret_cast<const u32x2 *>(raw + k_at + j * 4 * D + i * 32);
                     c = mma(widen8(w[0], w[1], 1.0f), qf[i], c);
                 }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[4 * j + i] = c[i];
         }
-        __builtin_amdgcn_sched_barrier(0);
-        load_k(t0 + 4 * kStep, pk);  // past the end: some page's codes, not used
-        pv = pv_next;
-        ksb = p.c.ks[safe(pv) * p.c.heads + head];
-        vsb = p.c.vs[safe(pv) * p.c.heads + head];
-        pk = page_of(t0 + 8 * kStep + tko);
-        pv_next = page_of(t0 + 8 * kStep + tvo);
+        // the next step's scales, pages of the one after, then its K into the place that has been read
+        own = UP ? page_at(kid[0], t0 + NW * kStep) : page_at(own_next, tv + NW * kStep);
+        uint32_t ksb = scale_of(p.c.ks, own), vsb = scale_of(p.c.vs, own);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        fetch_k(t0 + NW * kStep);  // past the end: some page's codes, not used
         const bool whole = t0 >= see_lo && t0 >= t_hi - (p.window > 0 ? p.window - 1 : INT32_MAX - 1) &&
                            t0 + kStep - 1 <= t_lo && t0 + kStep <= most;
         const bool every = __builtin_amdgcn_ballot_w64(!in) == 0 && whole;  // nothing masked in this step
@@ -453,21 +533,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
             s[i] *= ks;
         }
         if (!every) {
-            // codes that no row sees read as zero, and so do NaN codes, for now (nan_dims)
-            const int lo = in ? vis_lo - tv : 16, hi = vis_hi - tv;
+            const uint32_t vis = in ? seen16(vis_lo - tv, vis_hi - tv) : 0u;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = i >= lo && i < hi ? s[i] : -INFINITY;
-            uint32_t keep[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) keep[i] = byte_mask(tv + 4 * i, see_lo, in ? see_hi : 0);
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t u = vw[d][i] & keep[i], bad = nan_bytes(u);
-                    vw[d][i] = u & ~(bad * 0xffu);
-                    nans |= bad;
-                }
+            for (int i = 0; i < 16; ++i) s[i] = keep_seen(s[i], vis, i);
         }
         float top = s[0];
 #pragma unroll
@@ -499,6 +567,32 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
                 const float a = s[8 * u + 2 * i], c = s[8 * u + 2 * i + 1];
                 pf[u][i] = BF ? pair_near(a, c) : pair_cut(term_of(a, term), term_of(c, term));
             }
+        // this step's V is there, and so are the next one's scales (its K may be on its way)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::PASSES) : "memory");
+        if (!UP) asm volatile("" : "+v"(ksb), "+v"(vsb));  // taken here, not after the copies that follow
+        ks_next = e8m0(ksb) * scale;
+        vs_next = own >= 0 ? e8m0(vsb) : 1.0f;  // an absent page's byte may be any
+        u32x4 vw[DT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vw[d] = *reinterpret_cast<const u32x4 *>(raw + v_at + d * 1024);
+        ids(t0 + 2 * NW * kStep);
+        if (!UP) own_next = entry(t0 + 2 * NW * kStep + tvo);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        fetch_v(t0 + NW * kStep, vid_next);
+        if (!every) {
+            // codes that no row sees read as zero, and so do NaN codes, for now (nan_dims)
+            uint32_t keep[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) keep[i] = byte_mask(tv + 4 * i, see_lo, in ? see_hi : 0);
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t u = vw[d][i] & keep[i], bad = nan_bytes(u);
+                    vw[d][i] = u & ~(bad * 0xffu);
+                    nans |= bad;
+                }
+        }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const u32x4 v = vw[d];
@@ -522,9 +616,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
             for (int i = 0; i < 4; ++i) o[d][i] = (bits >> (4 * d + i)) & 1 ? NAN : o[d][i];
     }
 
-    // join the 4 waves: lanes of the tile's rows put their part down, wave w takes dims w * D / 4 ..
-    __shared__ float ml[4][16][2];
-    __shared__ float ow[4][R][D + 4];
+    // join the waves: lanes of the tile's rows put their part down
+    float(*ml)[16][2] = reinterpret_cast<float(*)[16][2]>(lds);
+    float(*ow)[R][D + 4] = reinterpret_cast<float(*)[R][D + 4]>(lds + NW * 16 * 2 * 4);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // every wave is done with its codes
     if (quad == 0) {
         ml[wave][col][0] = m;
         ml[wave][col][1] = sum;
@@ -534,16 +630,16 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
         for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(&ow[wave][col][d * 16 + quad * 4]) = o[d];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < here * D; i += 256) {
+    for (int i = threadIdx.x; i < here * D; i += NT) {
         const int row = i / D, d = i - row * D;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][row][0]);
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w][row][0]);
         // a NaN score leaves its row's sum NaN, whatever the maximum
         const float ref = top == -INFINITY ? 0.0f : top;
         float val = 0.0f, tot = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = __builtin_amdgcn_exp2f(ml[w][row][0] - ref);
             val += f * ow[w][row][d];
             tot += f * ml[w][row][1];
@@ -706,9 +802,21 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
     const float scale = p.scale * kLog2e;
     const int64_t page_bytes = (int64_t)P * D, stride = page_bytes * p.c.heads;
     const uint8_t *const kh = p.c.k + head * page_bytes, *const vh = p.c.v + head * page_bytes;
-    auto page_of = [&](int t) -> int {  // no branch: past the table, its last entry is read and not taken
-        const int id = table[min(t, most - 1) >> lgp];
-        return t < most && (uint32_t)id < (uint32_t)p.c.pages ? id : -1;
+    // A table entry as it is, and what it names for token t.  Through vector registers a use waits for every copy asked
+    // for before too, so that entries and scales are asked for a step ahead; where all lanes want the same one, it
+    // comes through the scalar cache, which counts apart.
+    auto entry = [&](int t) -> int {
+        const int32_t *at = table + (min(t, most - 1) >> lgp);
+        return UP ? (int)scalar_load(at) : *at;
+    };
+    auto page_at = [&](int id, int t) -> int { return t < most && (uint32_t)id < (uint32_t)p.c.pages ? id : -1; };
+    auto scale_of = [&](const uint8_t *scales, int page) -> uint32_t {
+        const uint8_t *at = scales + max(page, 0) * (int64_t)p.c.heads + head;
+        if constexpr (UP) {  // the dword that holds the byte
+            const uint64_t a = reinterpret_cast<uint64_t>(at);
+            return (scalar_load(reinterpret_cast<const void *>(a & ~3ull)) >> (8 * (a & 3))) & 255u;
+        }
+        return *at;
     };
     int kt[T::PASSES], ko[T::PASSES], vo[T::PASSES];  // token row; offsets within the step of a K and a V piece
     const int vc = threadIdx.x & 3;                   // a V piece's 16 tokens
@@ -720,29 +828,32 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
         vo[i] = (at >> 2) * P + vc * 16;
     }
     constexpr int IDS = UP ? 1 : T::PASSES;
-    int kid[IDS], vid;
+    int kid[IDS], vid = 0;  // table entries of the step that is fetched next
     auto ids = [&](int t0) {
         if constexpr (UP) {
-            kid[0] = vid = page_of(t0);
+            kid[0] = entry(t0);  // one register for all uses: a copy would wait for the load
         } else {
 #pragma unroll
-            for (int i = 0; i < IDS; ++i) kid[i] = page_of(t0 + min(kt[i], kStep - 1));
-            vid = page_of(t0 + 16 * vc);
+            for (int i = 0; i < IDS; ++i) kid[i] = entry(t0 + min(kt[i], kStep - 1));
+            vid = entry(t0 + 16 * vc);
         }
     };
     auto live = [&](int i) {  // a last pass may be the first waves' only
         return !(kStep * T::KC % 256) || i < T::PASSES - 1 || wave * 64 < kStep * T::KC % 256;
     };
-    auto fetch = [&](int t0, char *buf) {
+    struct Ids {
+        int k[IDS], v;
+    };
+    auto fetch = [&](const Ids &id, int t0, char *buf) {
         const int in = t0 & (P - 1);
 #pragma unroll
         for (int i = 0; i < T::PASSES; ++i) {
             if (!live(i)) break;
-            const uint8_t *k = UP ? kh + max(kid[0], 0) * stride + in * D + ko[i]
-                                  : kh + max(kid[UP ? 0 : i], 0) * stride + (((t0 + kt[i]) & (P - 1)) - kt[i]) * D + ko[i];
+            const int64_t page = max(page_at(id.k[UP ? 0 : i], UP ? t0 : t0 + min(kt[i], kStep - 1)), 0);
+            const uint8_t *k = kh + page * stride + (UP ? in * D : (((t0 + kt[i]) & (P - 1)) - kt[i]) * D) + ko[i];
             lds_copy16(k, buf + (i * 256 + wave * 64) * 16);
         }
-        const uint8_t *v = vh + max(vid, 0) * stride + (UP ? in : ((t0 + 16 * vc) & (P - 1)) - 16 * vc);
+        const uint8_t *v = vh + max(page_at(id.v, UP ? t0 : t0 + 16 * vc), 0) * stride + (UP ? in : ((t0 + 16 * vc) & (P - 1)) - 16 * vc);
 #pragma unroll
         for (int i = 0; i < T::PASSES; ++i) {
             if (!live(i)) break;
@@ -769,26 +880,39 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
     const int v_at = col * 128 + ((quad ^ ((col >> 1) & 7)) * 16);
     int buf = 0;
     if (threadIdx.x == 0) nans = 0;
+    auto now_ids = [&]() {
+        Ids r;
+#pragma unroll
+        for (int i = 0; i < IDS; ++i) r.k[i] = kid[i];
+        r.v = UP ? kid[0] : vid;
+        return r;
+    };
+    // a step ahead: the scales of the V pieces and of this lane's own 16 tokens, and whether these are there
+    int v_page = -1, own = -1, own_next = -1;
+    float ks_next = 0.0f, vs_next = 1.0f;
     if (from < to) {
         ids(from);
-        fetch(from, lds);
+        v_page = UP ? page_at(kid[0], from) : page_at(vid, from + 16 * vc);
+        own = UP ? v_page : page_at(entry(from + 16 * quad), from + 16 * quad);
+        vs_next = v_page >= 0 ? e8m0(scale_of(p.c.vs, v_page)) : 1.0f;  // an absent page's byte may be any
+        ks_next = e8m0(scale_of(p.c.ks, own)) * scale;
+        fetch(now_ids(), from, lds);
+        ids(from + kStep);
+        if (!UP) own_next = entry(from + kStep + 16 * quad);
     }
-    // a step ahead: the scales of the V pieces and of this lane's own 16 tokens, and whether these are there
-    int vid_now = from < to ? vid : -1, own = UP ? vid_now : from < to ? page_of(from + 16 * quad) : -1;
-    uint32_t vsb = p.c.vs[max(vid_now, 0) * (int64_t)p.c.heads + head], ksb = p.c.ks[max(own, 0) * (int64_t)p.c.heads + head];
-    if (from < to) ids(from + kStep);
     for (int t0 = from; t0 < to; t0 += kStep) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         char *const raw = lds + buf * (2 * T::RAW);
-        if (t0 + kStep < to) fetch(t0 + kStep, lds + (buf ^ 1) * (2 * T::RAW));
-        const bool in = own >= 0, v_in = vid_now >= 0;
-        const float ks = e8m0(ksb) * scale, vs = v_in ? e8m0(vsb) : 1.0f;  // an absent page's byte may be any
-        vid_now = vid;
-        own = UP ? vid : page_of(t0 + kStep + 16 * quad);
-        vsb = p.c.vs[max(vid_now, 0) * (int64_t)p.c.heads + head];
-        ksb = p.c.ks[max(own, 0) * (int64_t)p.c.heads + head];
+        const bool in = own >= 0, v_in = v_page >= 0;
+        const float ks = ks_next, vs = vs_next;
+        const Ids id = now_ids();
+        v_page = UP ? page_at(kid[0], t0 + kStep) : page_at(vid, t0 + kStep + 16 * vc);
+        own = UP ? v_page : page_at(own_next, t0 + kStep + 16 * quad);
+        uint32_t vsb = scale_of(p.c.vs, v_page), ksb = scale_of(p.c.ks, own);
         ids(t0 + 2 * kStep);
+        if (!UP) own_next = entry(t0 + 2 * kStep + 16 * quad);
+        if (t0 + kStep < to) fetch(id, t0 + kStep, lds + (buf ^ 1) * (2 * T::RAW));
         const int tv = t0 + 16 * quad;
         const bool whole = t0 >= see_lo && t0 >= t_hi - (p.window > 0 ? p.window - 1 : INT32_MAX - 1) &&
                            t0 + kStep - 1 <= t_lo && t0 + kStep <= most;
@@ -868,9 +992,9 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
             if (!every) {
-                const int lo = in ? vis_lo[c] - tv : 16, hi = vis_hi[c] - tv;
+                const uint32_t vis = in ? seen16(vis_lo[c] - tv, vis_hi[c] - tv) : 0u;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[c][i >> 2][i & 3] = i >= lo && i < hi ? s[c][i >> 2][i & 3] : -INFINITY;
+                for (int i = 0; i < 16; ++i) s[c][i >> 2][i & 3] = keep_seen(s[c][i >> 2][i & 3], vis, i);
             }
             const float f = ks * qscale[c];
             float top = s[c][0][0];
@@ -904,6 +1028,9 @@ __global__ __launch_bounds__(256, D == 256 && !BF ? 1 : 2) void kv_tiles_kernel(
                 }
         }
         lds_barrier();  // V is there; the next step's codes stay in flight
+        if (!UP) asm volatile("" : "+v"(ksb), "+v"(vsb));  // taken here, not where the wait would be for the copies too
+        vs_next = v_page >= 0 ? e8m0(vsb) : 1.0f;
+        ks_next = e8m0(ksb) * scale;
         const char *vl = vbuf + v_at;
         const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
@@ -1056,7 +1183,10 @@ hipError_t attend(const KvAttend &p, const KvPlan &pl, void *workspace, hipStrea
 #define DMC_DIM(N)                                                                                                     \
     case N:                                                                                                            \
         if (pl.kind == 0) {                                                                                            \
-            kv_rows_kernel<N, BF><<<rows_grid, dim3(256), 0, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total); \
+            auto f = p.c.page >= kStep ? kv_rows_kernel<N, BF, true> : kv_rows_kernel<N, BF, false>;                   \
+            e = hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, KvRows<N>::LDS); \
+            if (e != hipSuccess) return e;                                                                             \
+            f<<<rows_grid, dim3(64 * KvRows<N>::NW), KvRows<N>::LDS, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total); \
         } else {                                                                                                       \
             auto f = p.c.page >= kStep ? kv_tiles_kernel<N, BF, kTiles<N, BF>, true> : kv_tiles_kernel<N, BF, kTiles<N, BF>, false>; \
             e = hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, KvTile<N>::LDS); \
