@@ -43,6 +43,7 @@ struct MxProblem {
 struct MxPlan {
     int kind;        // 0: rows (f32 x, few activation rows), 1: tiles
     int tiles;       // rows: 16-row weight tiles per workgroup
+    int steps;       // rows: groups of 128 k that a wave takes of each
     int shape;       // tiles: which tile shape
     int slices, per; // tiles: slices of k, groups of 128 in each
     int64_t grid_x;

@@ -303,9 +303,10 @@ __device__ __forceinline__ uint64_t nan_dims(const KvAttend &p, const int32_t *t
     return bits;
 }
 
+template <bool NT = false>  // NT: read once, not to be kept in the caches
 __device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i's 16 bytes to l + 16 i
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
-                                     (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
+                                     (__attribute__((address_space(3))) uint32_t *)l, 16, 0, NT ? kLoadNT : 0);
 }
 
 // Bits lo .. hi - 1 of 16, and a score where its bit is set, else -inf (by bits: 16 lane masks would not fit the
@@ -359,7 +360,9 @@ struct KvRows {
     }
 };
 
-template <int D, bool BF, bool UP>
+// ONCE: one column tile, so that no other workgroup reads the same codes.  Measured on 64 sequences up to 8192: 153 us
+// with the codes kept in the caches, 144 without.
+template <int D, bool BF, bool UP, bool ONCE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const KvAttend p, const KvPart part, int splits, int chunk,
                                                                         int row_tiles, int64_t rows_total) {
     using T = KvRows<D>;
@@ -436,18 +439,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
         for (int i = 0; i < T::PASSES; ++i) {
             const int at = i * 64 + lane, t = at / T::KC, off = t * D + ((at % T::KC) ^ T::k_key(t)) * 16;
             if constexpr (UP) {
-                lds_copy16(kh + max(page_at(kid[0], t0), 0) * stride + in * D + off, mine + i * 1024);
+                lds_copy16<ONCE>(kh + max(page_at(kid[0], t0), 0) * stride + in * D + off, mine + i * 1024);
             } else {
                 const int g = t >> 4;
                 const int id = D != 96 ? kid[(i * 64 / T::KC) >> 4] : g == 0 ? kid[0] : g == 1 ? kid[1] : g == 2 ? kid[2] : kid[3];
-                lds_copy16(kh + max(page_at(id, t0 + 16 * g), 0) * stride + (((t0 + 16 * g) & (P - 1)) - 16 * g) * D + off, mine + i * 1024);
+                lds_copy16<ONCE>(kh + max(page_at(id, t0 + 16 * g), 0) * stride + (((t0 + 16 * g) & (P - 1)) - 16 * g) * D + off, mine + i * 1024);
             }
         }
     };
     auto fetch_v = [&](int t0, int id) {
         const uint8_t *v = vh + max(page_at(id, UP ? t0 : t0 + 16 * vc), 0) * stride + (UP ? t0 & (P - 1) : ((t0 + 16 * vc) & (P - 1)) - 16 * vc) + vo;
 #pragma unroll
-        for (int i = 0; i < T::PASSES; ++i) lds_copy16(v + i * 16 * P, mine + T::RAW + i * 1024);
+        for (int i = 0; i < T::PASSES; ++i) lds_copy16<ONCE>(v + i * 16 * P, mine + T::RAW + i * 1024);
     };
     const int first = from + wave * kStep, tvo = 16 * quad;
     int own = -1, own_next = -1;
@@ -1183,7 +1186,9 @@ hipError_t attend(const KvAttend &p, const KvPlan &pl, void *workspace, hipStrea
 #define DMC_DIM(N)                                                                                                     \
     case N:                                                                                                            \
         if (pl.kind == 0) {                                                                                            \
-            auto f = p.c.page >= kStep ? kv_rows_kernel<N, BF, true> : kv_rows_kernel<N, BF, false>;                   \
+            const bool up = p.c.page >= kStep, nt = row_tiles == 1;                                                    \
+            auto f = up ? (nt ? kv_rows_kernel<N, BF, true, true> : kv_rows_kernel<N, BF, true, false>)                \
+                        : (nt ? kv_rows_kernel<N, BF, false, true> : kv_rows_kernel<N, BF, false, false>);             \
             e = hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, KvRows<N>::LDS); \
             if (e != hipSuccess) return e;                                                                             \
             f<<<rows_grid, dim3(64 * KvRows<N>::NW), KvRows<N>::LDS, stream>>>(p, part, pl.splits, pl.chunk, row_tiles, rows_total); \
@@ -1240,9 +1245,13 @@ KvPlan plan_kv(const KvAttend &p, int num_cus) {
     int64_t span = p.b.max_len;
     if (p.window > 0) span = std::min<int64_t>(span, p.window + R + kStep);
     const int64_t units = std::max<int64_t>(1, (span + unit - 1) / unit);
-    const int64_t want = std::max<int64_t>(1, (pl.kind ? 2 : 8) * num_cus / std::max<int64_t>(1, tiles));
-    // steps per workgroup: a split of few costs more in its partial results than it saves
-    const int64_t per = std::max<int64_t>((units + want - 1) / want, std::max<int64_t>(pl.kind ? 8 : 4, (units + kMaxSplits - 1) / kMaxSplits));
+    // Few rows: one workgroup per CU, each as long as that allows up to 16 steps of 256 tokens (uneven sequences then
+    // still spread).  One token over 131072: 16 steps 61 us, 8 65, 4 75, 2 97; 64 sequences up to 8192: 144, 153, 153.
+    // Tiles: two per CU, of at least 8 steps, since each writes its partial rows.
+    const int64_t want = std::max<int64_t>(1, (pl.kind ? 2 : 1) * num_cus / std::max<int64_t>(1, tiles));
+    int64_t per = (units + want - 1) / want;
+    per = pl.kind ? std::max<int64_t>(per, 8) : std::min<int64_t>(per, 16);
+    per = std::max<int64_t>(per, (units + kMaxSplits - 1) / kMaxSplits);
     pl.chunk = (int)(per * unit);
     pl.splits = (int)((units + per - 1) / per);
     if (pl.splits > 1)

@@ -177,62 +177,78 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t *__re
 // only their f32 sums round.  The 3 m terms are columns of one 16-wide tile.
 //
 // A workgroup of 8 waves owns T tiles of 16 weight rows and walks k in chunks of
-// 4096: the terms of x go to LDS once per chunk, each wave takes 512 k of every
-// tile, and the waves' sums meet in LDS at the end, in wave order.
+// 8 * S * 128: the terms of x go to LDS once per chunk, each wave takes S groups of
+// every tile, and the waves' sums meet in LDS at the end, in wave order.  S follows
+// the length of the rows, so that short ones still keep every wave at work.
+//
+// What bounds it: weights straight from HBM; a lane reads 16 bytes of its own row, 64
+// accesses of the L1 per KB, which at 2.4 GHz is 9.8 TB/s of codes.  Scales come in one
+// load of S dwords per row and chunk for the same reason.
 constexpr int kRowsWaves = 8;
-constexpr int kRowsSteps = 4;                              // groups of 128 per wave and chunk
-constexpr int kRowsChunk = kRowsWaves * kRowsSteps * 128;  // 4096
-constexpr int kRowsMax = 5;                                // activation rows: 3 terms each in 16 columns
-constexpr int kRowsLds = kRowsChunk * 2 + 64;              // bytes of one term's chunk; 64 shift the banks
+constexpr int kRowsMax = 5;  // activation rows: 3 terms each in 16 columns
+constexpr int rows_chunk(int steps) { return kRowsWaves * steps * 128; }
+constexpr int rows_pitch(int steps) { return rows_chunk(steps) * 2 + 64; }  // bytes of one term's chunk; 64 shift the banks
 
 __device__ __forceinline__ uint32_t cut2(float a, float b) {  // bf16 pair of two values' upper halves
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 
+template <int S>
 struct MxStep {
-    u32x4 w;
-    uint32_t s;
+    u32x4 w[S];
+    uint32_t s[S];
 };
 
-template <int T>
+template <int T, int S>
 __global__ __launch_bounds__(512) void mx_rows_kernel(const float *__restrict__ x, const uint8_t *__restrict__ wq,
                                                       const uint8_t *__restrict__ ws, float *__restrict__ y, int m,
                                                       int k, int n) {
+    constexpr int kChunk = rows_chunk(S), kPitch = rows_pitch(S);
     extern __shared__ char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, quad = lane >> 4;
     const int groups = (k + 127) >> 7, cols = 3 * m;
     const int64_t row0 = (int64_t)blockIdx.x * T * 16;
-    const int chunks = (groups + kRowsWaves * kRowsSteps - 1) / (kRowsWaves * kRowsSteps);
+    const int chunks = (groups + kRowsWaves * S - 1) / (kRowsWaves * S);
     const uint32_t qrow = (uint32_t)groups * 64u, srow = (uint32_t)groups * 4u;
 
-    auto load = [&](MxStep *st, int t, int chunk) {
+    auto load = [&](MxStep<S> &st, int t, int chunk) {
         const int64_t at = row0 + t * 16;
         const int64_t left = max((int64_t)0, min((int64_t)16, (int64_t)n - at));
         const __amdgpu_buffer_rsrc_t qr = weight_rsrc(wq + at * qrow, (uint32_t)left * qrow);
         const __amdgpu_buffer_rsrc_t sr = weight_rsrc(ws + at * srow, (uint32_t)left * srow);
+        const int g0 = (chunk * kRowsWaves + wave) * S;
+        const uint32_t so = g0 < groups ? (uint32_t)r * srow + (uint32_t)g0 * 4u : 0xfffffff0u;
+        if constexpr (S == 4) {
+            const u32x4 s = __builtin_amdgcn_raw_buffer_load_b128(sr, so, 0, 0);
 #pragma unroll
-        for (int i = 0; i < kRowsSteps; ++i) {
-            // past the row's end there is the next row: read as zeros instead
-            const int g = chunk * kRowsWaves * kRowsSteps + wave * kRowsSteps + i;
-            const uint32_t qo = g < groups ? (uint32_t)r * qrow + (uint32_t)g * 64u + quad * 16u : 0xfffffff0u;
-            const uint32_t so = g < groups ? (uint32_t)r * srow + (uint32_t)g * 4u : 0xfffffff0u;
-            st[i].w = load_w16(qr, qo);
-            st[i].s = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(sr, so, 0, kLoadNT);
+            for (int i = 0; i < S; ++i) st.s[i] = s[i];
+        } else if constexpr (S == 2) {
+            const u32x2 s = __builtin_amdgcn_raw_buffer_load_b64(sr, so, 0, 0);
+            st.s[0] = s[0];
+            st.s[1] = s[1];
+        } else {
+            st.s[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(sr, so, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            // past the row's end there is the next row: codes read as zeros (their scales are not used, multiply)
+            const uint32_t qo = g0 + i < groups ? (uint32_t)r * qrow + (uint32_t)(g0 + i) * 64u + quad * 16u : 0xfffffff0u;
+            st.w[i] = load_w16(qr, qo);
         }
     };
 
     f32x4 acc[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) acc[t] = f32x4{0, 0, 0, 0};
-    MxStep now[kRowsSteps];
+    MxStep<S> now;
     load(now, 0, 0);
-    const char *xc = lds + min(r, cols - 1) * kRowsLds + wave * (kRowsSteps * 256) + quad * 64;
+    const char *xc = lds + min(r, cols - 1) * kPitch + wave * (S * 256) + quad * 64;
     for (int c = 0; c < chunks; ++c) {
         if (c) __syncthreads();
-        for (int i = threadIdx.x; i < m * (kRowsChunk / 8); i += 512) {
-            const int row = i / (kRowsChunk / 8), at = (i - row * (kRowsChunk / 8)) * 8;
-            const int k0 = c * kRowsChunk + at;
+        for (int i = threadIdx.x; i < m * (kChunk / 8); i += 512) {
+            const int row = i / (kChunk / 8), at = (i - row * (kChunk / 8)) * 8;
+            const int k0 = c * kChunk + at;
             MxIn<false> v;
             v.load(x, (int64_t)row * k + k0, max(0, k - k0));
             u32x4 term[3];
@@ -254,34 +270,33 @@ __global__ __launch_bounds__(512) void mx_rows_kernel(const float *__restrict__ 
                 term[2][j] = cut2(d[0], d[1]);
             }
 #pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(lds + (row * 3 + p) * kRowsLds + at * 2) = term[p];
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(lds + (row * 3 + p) * kPitch + at * 2) = term[p];
         }
         __syncthreads();
+        const int g0 = (c * kRowsWaves + wave) * S;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
             // the next tile's weights (past the last chunk: zeros, unread)
-            MxStep next[kRowsSteps];
+            MxStep<S> next;
             load(next, t < T - 1 ? t + 1 : 0, t < T - 1 ? c : c + 1);
 #pragma unroll
-            for (int i = 0; i < kRowsSteps; ++i) {
-                const float sc = e8m0((now[i].s >> (8 * quad)) & 255u);
+            for (int i = 0; i < S; ++i) {
+                const uint32_t byte = g0 + i < groups ? (now.s[i] >> (8 * quad)) & 255u : 127u;
+                const float sc = e8m0(byte);
                 const char *xb = xc + i * 256;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t w = now[i].w[j];
+                    const uint32_t w = now.w[i][j];
                     u32x4 a;
                     a[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
                     a[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
                     a[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
                     a[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
                     const u32x4 b = *reinterpret_cast<const u32x4 *>(xb + j * 16);
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                                     __builtin_bit_cast(bf16x8, b),
-                                                                     acc[t], 0, 0, 0);
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc[t], 0, 0, 0);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < kRowsSteps; ++i) now[i] = next[i];
+            now = next;
         }
     }
     __syncthreads();
@@ -303,8 +318,13 @@ __global__ __launch_bounds__(512) void mx_rows_kernel(const float *__restrict__ 
     }
 }
 
-size_t rows_lds(int tiles, int m) {
-    return std::max((size_t)3 * m * kRowsLds, (size_t)tiles * kRowsWaves * 16 * 16 * 4);
+size_t rows_lds(int tiles, int steps, int m) {
+    return std::max((size_t)3 * m * rows_pitch(steps), (size_t)tiles * kRowsWaves * 16 * 16 * 4);
+}
+
+template <int T>
+auto rows_kernel(int steps) {
+    return steps == 4 ? mx_rows_kernel<T, 4> : steps == 2 ? mx_rows_kernel<T, 2> : mx_rows_kernel<T, 1>;
 }
 
 // ---- product, tiles ---------------------------------------------------------------
@@ -684,7 +704,9 @@ MxPlan plan_mx(const MxProblem &p, int num_cus) {
     if (p.x && p.m <= kRowsMax) {
         pl.kind = 0;
         const int64_t tiles = (p.n + 15) / 16;
-        pl.tiles = tiles >= 8 * 4 * (int64_t)num_cus ? 8 : tiles >= 2 * 4 * (int64_t)num_cus ? 2 : 1;
+        pl.tiles = tiles >= 8 * 2 * (int64_t)num_cus ? 8 : tiles >= 2 * 4 * (int64_t)num_cus ? 2 : 1;
+        const int64_t each = (mx_groups(p.k) + kRowsWaves - 1) / kRowsWaves;  // groups of a wave
+        pl.steps = each > 2 ? 4 : each > 1 ? 2 : 1;
         pl.grid_x = (tiles + pl.tiles - 1) / pl.tiles;
         return pl;
     }
@@ -713,8 +735,8 @@ hipError_t launch_mx(const MxProblem &p, const MxPlan &pl, void *workspace, hipS
         return hipGetLastError();
     }
     if (pl.kind == 0) {
-        const size_t lds = rows_lds(pl.tiles, (int)p.m);
-        auto f = pl.tiles == 8 ? mx_rows_kernel<8> : pl.tiles == 2 ? mx_rows_kernel<2> : mx_rows_kernel<1>;
+        const size_t lds = rows_lds(pl.tiles, pl.steps, (int)p.m);
+        auto f = pl.tiles == 8 ? rows_kernel<8>(pl.steps) : pl.tiles == 2 ? rows_kernel<2>(pl.steps) : rows_kernel<1>(pl.steps);
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
         if (e != hipSuccess) return e;
         f<<<dim3((unsigned)pl.grid_x), dim3(512), lds, stream>>>(p.x, p.wq, p.ws, p.y, (int)p.m, (int)p.k, (int)p.n);
