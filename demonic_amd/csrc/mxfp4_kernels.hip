@@ -169,9 +169,18 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t *__re
     }
 }
 
+__device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i's 16 bytes to l + 16 i
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
+                                     (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
+}
+__device__ __forceinline__ void lds_copy4(const void *g, char *l) {  // lane i's 4 bytes to l + 4 i
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
+                                     (__attribute__((address_space(3))) uint32_t *)l, 4, 0, 0);
+}
+
 // ---- product, few activation rows ------------------------------------------------
 //
-// y = x W' with x f32 and at most 5 rows.  Each activation is the sum of three
+// y = x W' with x f32 and at most 2 rows.  Each activation is the sum of three
 // bf16 terms (8 + 8 + 8 bits of its 24, cut, so the sum is exact); a code times
 // its scale is exact in bf16 too; so the matrix cores' products are exact and
 // only their f32 sums round.  The 3 m terms are columns of one 16-wide tile.
@@ -181,71 +190,67 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t *__re
 // every tile, and the waves' sums meet in LDS at the end, in wave order.  S follows
 // the length of the rows, so that short ones still keep every wave at work.
 //
-// What bounds it: weights straight from HBM; a lane reads 16 bytes of its own row, 64
-// accesses of the L1 per KB, which at 2.4 GHz is 9.8 TB/s of codes.  Scales come in one
-// load of S dwords per row and chunk for the same reason.
+// What bounds it: weights straight from HBM.  A wave's codes and scales go to LDS of its
+// own, two tiles ahead and without passing through registers, by copies whose lanes take
+// whole row pieces (lanes that read 16 bytes of different rows each cost the L1 an
+// access: m = 1 on [14336,4096] took 10.9 us that way, on [128256,4096] 79).
 constexpr int kRowsWaves = 8;
-constexpr int kRowsMax = 5;  // activation rows: 3 terms each in 16 columns
+constexpr int kRowsMax = 2;   // activation rows: 3 terms each in 16 columns; more do not fit the LDS beside the weights
+constexpr int kRowsDepth = 3;  // tiles on their way or in use
 constexpr int rows_chunk(int steps) { return kRowsWaves * steps * 128; }
 constexpr int rows_pitch(int steps) { return rows_chunk(steps) * 2 + 64; }  // bytes of one term's chunk; 64 shift the banks
+constexpr int rows_item(int steps) { return steps * 1024 + 256; }           // bytes of a wave's codes and scales of a tile
 
 __device__ __forceinline__ uint32_t cut2(float a, float b) {  // bf16 pair of two values' upper halves
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 
-template <int S>
-struct MxStep {
-    u32x4 w[S];
-    uint32_t s[S];
-};
+__device__ __forceinline__ void lds_barrier() {  // for LDS alone: copies in flight stay so
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 template <int T, int S>
 __global__ __launch_bounds__(512) void mx_rows_kernel(const float *__restrict__ x, const uint8_t *__restrict__ wq,
                                                       const uint8_t *__restrict__ ws, float *__restrict__ y, int m,
                                                       int k, int n) {
-    constexpr int kChunk = rows_chunk(S), kPitch = rows_pitch(S);
-    extern __shared__ char lds[];
+    constexpr int kChunk = rows_chunk(S), kPitch = rows_pitch(S), kItem = rows_item(S);
+    constexpr int kPer = 16 / S;  // rows of a copy
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, quad = lane >> 4;
     const int groups = (k + 127) >> 7, cols = 3 * m;
     const int64_t row0 = (int64_t)blockIdx.x * T * 16;
-    const int chunks = (groups + kRowsWaves * S - 1) / (kRowsWaves * S);
-    const uint32_t qrow = (uint32_t)groups * 64u, srow = (uint32_t)groups * 4u;
+    const int chunks = (groups + kRowsWaves * S - 1) / (kRowsWaves * S), items = chunks * T;
+    const int64_t qrow = (int64_t)groups * 64, srow = (int64_t)groups * 4;
+    char *const mine = lds + wave * (kRowsDepth * kItem), *const terms = lds + kRowsWaves * kRowsDepth * kItem;
+    // 16-byte piece p of row r lies at place p ^ key(r): an operand read takes 16 rows' pieces, none in another's bank
+    auto key = [](int row) { return S == 4 ? row & 15 : (row >> 1) & (4 * S - 1); };
 
-    auto load = [&](MxStep<S> &st, int t, int chunk) {
-        const int64_t at = row0 + t * 16;
-        const int64_t left = max((int64_t)0, min((int64_t)16, (int64_t)n - at));
-        const __amdgpu_buffer_rsrc_t qr = weight_rsrc(wq + at * qrow, (uint32_t)left * qrow);
-        const __amdgpu_buffer_rsrc_t sr = weight_rsrc(ws + at * srow, (uint32_t)left * srow);
-        const int g0 = (chunk * kRowsWaves + wave) * S;
-        const uint32_t so = g0 < groups ? (uint32_t)r * srow + (uint32_t)g0 * 4u : 0xfffffff0u;
-        if constexpr (S == 4) {
-            const u32x4 s = __builtin_amdgcn_raw_buffer_load_b128(sr, so, 0, 0);
+    // Item i: tile i % T of chunk i / T.  Rows past the last are the last again, and so are groups (not multiplied).
+    auto fetch = [&](int i) {
+        if (i >= items) i = items - 1;  // always the same number of copies
+        const int c = i / T, t = i - c * T, g0 = (c * kRowsWaves + wave) * S;
+        char *const to = mine + (i % kRowsDepth) * kItem;
 #pragma unroll
-            for (int i = 0; i < S; ++i) st.s[i] = s[i];
-        } else if constexpr (S == 2) {
-            const u32x2 s = __builtin_amdgcn_raw_buffer_load_b64(sr, so, 0, 0);
-            st.s[0] = s[0];
-            st.s[1] = s[1];
-        } else {
-            st.s[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(sr, so, 0, 0);
+        for (int j = 0; j < S; ++j) {
+            const int row = j * kPer + lane / (4 * S), piece = (lane & (4 * S - 1)) ^ key(row);
+            const int at = min(g0 * 64 + piece * 16, (groups - 1) * 64 + (piece & 3) * 16);
+            lds_copy16(wq + min(row0 + t * 16 + row, (int64_t)n - 1) * qrow + at, to + j * 1024);
         }
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            // past the row's end there is the next row: codes read as zeros (their scales are not used, multiply)
-            const uint32_t qo = g0 + i < groups ? (uint32_t)r * qrow + (uint32_t)(g0 + i) * 64u + quad * 16u : 0xfffffff0u;
-            st.w[i] = load_w16(qr, qo);
-        }
+        const int row = (lane / S) & 15;
+        lds_copy4(ws + min(row0 + t * 16 + row, (int64_t)n - 1) * srow + min(g0 + lane % S, groups - 1) * 4, to + S * 1024);
     };
 
     f32x4 acc[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) acc[t] = f32x4{0, 0, 0, 0};
-    MxStep<S> now;
-    load(now, 0, 0);
-    const char *xc = lds + min(r, cols - 1) * kPitch + wave * (S * 256) + quad * 64;
+    fetch(0);
+    fetch(1);
+    const char *xc = terms + min(r, cols - 1) * kPitch + wave * (S * 256) + quad * 64;
     for (int c = 0; c < chunks; ++c) {
-        if (c) __syncthreads();
+        if (c) lds_barrier();
         for (int i = threadIdx.x; i < m * (kChunk / 8); i += 512) {
             const int row = i / (kChunk / 8), at = (i - row * (kChunk / 8)) * 8;
             const int k0 = c * kChunk + at;
@@ -270,35 +275,39 @@ __global__ __launch_bounds__(512) void mx_rows_kernel(const float *__restrict__ 
                 term[2][j] = cut2(d[0], d[1]);
             }
 #pragma unroll
-            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(lds + (row * 3 + p) * kPitch + at * 2) = term[p];
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x4 *>(terms + (row * 3 + p) * kPitch + at * 2) = term[p];
         }
-        __syncthreads();
+        lds_barrier();
         const int g0 = (c * kRowsWaves + wave) * S;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            // the next tile's weights (past the last chunk: zeros, unread)
-            MxStep<S> next;
-            load(next, t < T - 1 ? t + 1 : 0, t < T - 1 ? c : c + 1);
+            // this wave's reads of the place that is filled next are done, and this tile's copies (two tiles' after it
+            // may be on their way)
+            const int i = c * T + t;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            fetch(i + 2);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (S + 1)) : "memory");
+            const char *at = mine + (i % kRowsDepth) * kItem;
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const uint32_t byte = g0 + i < groups ? (now.s[i] >> (8 * quad)) & 255u : 127u;
-                const float sc = e8m0(byte);
-                const char *xb = xc + i * 256;
+            for (int s = 0; s < S; ++s) {
+                if (g0 + s >= groups) break;
+                const u32x4 w = *reinterpret_cast<const u32x4 *>(at + r * (64 * S) + (((4 * s + quad) ^ key(r)) * 16));
+                const float sc = e8m0(*reinterpret_cast<const uint8_t *>(at + S * 1024 + (r * S + s) * 4 + quad));
+                const char *xb = xc + s * 256;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t w = now.w[i][j];
                     u32x4 a;
-                    a[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0));
-                    a[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1));
-                    a[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2));
-                    a[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3));
+                    a[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], sc, 0));
+                    a[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], sc, 1));
+                    a[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], sc, 2));
+                    a[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j], sc, 3));
                     const u32x4 b = *reinterpret_cast<const u32x4 *>(xb + j * 16);
                     acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc[t], 0, 0, 0);
                 }
             }
-            now = next;
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy lands on the sums
     __syncthreads();
     float *red = reinterpret_cast<float *>(lds);  // [T][wave][col][16 rows]
 #pragma unroll
@@ -319,7 +328,8 @@ __global__ __launch_bounds__(512) void mx_rows_kernel(const float *__restrict__ 
 }
 
 size_t rows_lds(int tiles, int steps, int m) {
-    return std::max((size_t)3 * m * rows_pitch(steps), (size_t)tiles * kRowsWaves * 16 * 16 * 4);
+    return std::max((size_t)kRowsWaves * kRowsDepth * rows_item(steps) + (size_t)3 * m * rows_pitch(steps),
+                    (size_t)tiles * kRowsWaves * 16 * 16 * 4);
 }
 
 template <int T>
@@ -413,15 +423,6 @@ struct MxTileArgs {
     int slices, per;           // slices of k, groups of each
     bool wide_scales;          // rows of scales are 16-byte aligned, slices too
 };
-
-__device__ __forceinline__ void lds_copy16(const void *g, char *l) {  // lane i's 16 bytes to l + 16 i
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
-                                     (__attribute__((address_space(3))) uint32_t *)l, 16, 0, 0);
-}
-__device__ __forceinline__ void lds_copy4(const void *g, char *l) {  // lane i's 4 bytes to l + 4 i
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)g,
-                                     (__attribute__((address_space(3))) uint32_t *)l, 4, 0, 0);
-}
 
 // Tiles of TN weight rows x TM activation rows; WN x WM waves of RT x CT MFMA tiles.  Both sides go to LDS without
 // passing through registers, SK groups of 128 k per stage, three stages deep.
@@ -671,9 +672,9 @@ hipError_t launch_mx_dequantize(const MxCast &p, hipStream_t stream) {
     X(6, kDigits, 4, 1, 4, 1, 2) /* 256 x 16 */
 
 namespace {
-struct Shape { int tn, tm; };
+struct Shape { int tn, tm, lds; };
 constexpr Shape kShapes[] = {
-#define X(ID, PL, RT, CT, WN, WM, SK) {WN * RT * 16, WM * CT * 16},
+#define X(ID, PL, RT, CT, WN, WM, SK) {WN * RT * 16, WM * CT * 16, MxTile<PL, RT, CT, WN, WM, SK>::kLds},
     DMC_MX_SHAPES(X)
 #undef X
 };
@@ -704,7 +705,9 @@ MxPlan plan_mx(const MxProblem &p, int num_cus) {
     if (p.x && p.m <= kRowsMax) {
         pl.kind = 0;
         const int64_t tiles = (p.n + 15) / 16;
-        pl.tiles = tiles >= 8 * 2 * (int64_t)num_cus ? 8 : tiles >= 2 * 4 * (int64_t)num_cus ? 2 : 1;
+        // one workgroup per CU (what their LDS allows) as far as 16 tiles each go: m = 1 on [14336,4096] 9.6 us with 4
+        // tiles, 16.1 with 2; on [128256,4096] 57.7 with 16, 61.1 with 8
+        pl.tiles = tiles > 8 * (int64_t)num_cus ? 16 : tiles > 4 * (int64_t)num_cus ? 8 : tiles > 2 * (int64_t)num_cus ? 4 : tiles > num_cus ? 2 : 1;
         const int64_t each = (mx_groups(p.k) + kRowsWaves - 1) / kRowsWaves;  // groups of a wave
         pl.steps = each > 2 ? 4 : each > 1 ? 2 : 1;
         pl.grid_x = (tiles + pl.tiles - 1) / pl.tiles;
@@ -716,11 +719,14 @@ MxPlan plan_mx(const MxProblem &p, int num_cus) {
     else pl.shape = p.m > 32 ? 3 : p.m > 16 ? 4 : p.n >= 256 * (int64_t)num_cus ? 6 : 5;
     const Shape s = kShapes[pl.shape];
     pl.grid_x = (int64_t)div_up(p.n, s.tn) * div_up(p.m, s.tm);
-    // k is cut where the tiles alone leave CUs without one
+    // k is cut, into slices of 8 groups or more, where the tiles alone leave room on the CUs: f32 x two workgroups per
+    // CU where the LDS holds them (m = 11 on [7040,10752]: 21.2 us, one per CU 24.3), x in MXFP4 one (m = 1 on
+    // [14336,4096]: 7.8 us uncut, 10.4 with room for four)
+    const int64_t room = (int64_t)num_cus * (p.x ? std::min(2, 160 * 1024 / s.lds) : 1);
     pl.slices = 1;
-    if (pl.grid_x < num_cus) {
+    if (pl.grid_x * 2 <= room) {
         const int64_t most = std::max<int64_t>(1, groups / 8);
-        pl.slices = (int)std::min<int64_t>(most, num_cus / pl.grid_x);
+        pl.slices = (int)std::min<int64_t>(most, room / pl.grid_x);
     }
     pl.per = (int)((groups + pl.slices - 1) / pl.slices + 3) / 4 * 4;
     pl.slices = (int)((groups + pl.per - 1) / pl.per);
@@ -736,7 +742,11 @@ hipError_t launch_mx(const MxProblem &p, const MxPlan &pl, void *workspace, hipS
     }
     if (pl.kind == 0) {
         const size_t lds = rows_lds(pl.tiles, pl.steps, (int)p.m);
-        auto f = pl.tiles == 8 ? rows_kernel<8>(pl.steps) : pl.tiles == 2 ? rows_kernel<2>(pl.steps) : rows_kernel<1>(pl.steps);
+        auto f = pl.tiles == 16  ? rows_kernel<16>(pl.steps)
+                 : pl.tiles == 8 ? rows_kernel<8>(pl.steps)
+                 : pl.tiles == 4 ? rows_kernel<4>(pl.steps)
+                 : pl.tiles == 2 ? rows_kernel<2>(pl.steps)
+                                 : rows_kernel<1>(pl.steps);
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
         if (e != hipSuccess) return e;
         f<<<dim3((unsigned)pl.grid_x), dim3(512), lds, stream>>>(p.x, p.wq, p.ws, p.y, (int)p.m, (int)p.k, (int)p.n);

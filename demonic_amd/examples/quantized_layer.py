@@ -1,0 +1,111 @@
+"""One attention layer with 4-bit weights and an 8-bit cache, a prompt and then single tokens.
+
+    python -m demonic_amd.examples.quantized_layer [--hidden 1024 --steps 4]
+
+The stacked q/k/v projection and the output projection are quantised to MXFP4 once, on the device.  A prompt's rows
+go through the projection with 4-bit activations (gemm_mxfp4), its k and v into the cache's pages (kv8_append) and
+its q over them (kv8_attend); each further token does the same with f32 activations (gemv_mxfp4_rd), its step recorded
+as a graph.  Prints the time of the prompt and of a token (recording and copies from the host included) and the norm
+of the last output.
+"""
+from __future__ import annotations
+
+import argparse
+import time
+
+import numpy as np
+
+import demonic_amd as d
+
+
+class Layer:
+    """The layer's weights, pages and scratch on the device."""
+
+    def __init__(self, hidden: int, heads: int, kv_heads: int, dim: int, page: int, most: int, seed: int = 0):
+        self.hidden, self.heads, self.kv, self.dim = hidden, heads, kv_heads, dim
+        self.wide = (heads + 2 * kv_heads) * dim
+        rng = np.random.default_rng(seed)
+        self.w_qkv, self.qkv_scales = self._weight(rng, self.wide, hidden)
+        self.w_out, self.out_scales = self._weight(rng, hidden, heads * dim)
+        self.pages = -(-most // page)
+        side = self.pages * kv_heads * page * dim
+        self.buffers = [d.DeviceBuffer(n) for n in (side, side, self.pages * kv_heads, self.pages * kv_heads)]
+        self.cache = d.KV8Cache(*self.buffers, self.pages, kv_heads, page, dim)
+        # pages in an order of their own, as a pool hands them out
+        self.table = d.DeviceBuffer.from_numpy(rng.permutation(self.pages).astype(np.int32))
+        self.lens, self.starts = d.DeviceBuffer(4), d.DeviceBuffer(8)
+        self.x, self.qkv = d.DeviceBuffer(4 * most * hidden), d.DeviceBuffer(4 * most * self.wide)
+        self.heads_out, self.y = d.DeviceBuffer(4 * most * heads * dim), d.DeviceBuffer(4 * most * hidden)
+        qb, sb = d.mxfp4_row(hidden)
+        ob, os = d.mxfp4_row(heads * dim)
+        self.xq, self.xs = d.DeviceBuffer(most * max(qb, ob)), d.DeviceBuffer(most * max(sb, os))
+
+    def _weight(self, rng, n, k):
+        w = (0.02 * rng.standard_normal((n, k), dtype=np.float32))
+        qb, sb = d.mxfp4_row(k)
+        q, s = d.DeviceBuffer(n * qb), d.DeviceBuffer(n * sb)
+        with d.DeviceBuffer.from_numpy(w) as src:
+            d.mxfp4_quantize(src, q, s, n, k)
+            d.synchronize()
+        return q, s
+
+    def enqueue(self, rows: int, length: int, four_bits: bool) -> None:
+        """The layer on `rows` new tokens, `length` tokens with them: no host work between its launches."""
+        def product(x, w, scales, y, k, n):
+            if four_bits:
+                d.mxfp4_quantize(x, self.xq, self.xs, rows, k)
+                d.gemm_mxfp4(self.xq, self.xs, w, scales, y, rows, k, n)
+            else:
+                d.gemv_mxfp4_rd(x, w, scales, y, rows, k, n)
+
+        batch = d.KV8Batch(self.table, self.pages, self.lens, self.starts, 1, rows, length)
+        q, k = self.qkv.addr, self.qkv.addr + 4 * self.heads * self.dim
+        product(self.x, self.w_qkv, self.qkv_scales, self.qkv, self.hidden, self.wide)
+        d.kv8_append(self.cache, batch, k, k + 4 * self.kv * self.dim, k_ld=self.wide, v_ld=self.wide)
+        d.kv8_attend(self.cache, batch, q, self.heads_out, self.heads, q_ld=self.wide)
+        product(self.heads_out, self.w_out, self.out_scales, self.y, self.heads * self.dim, self.hidden)
+
+    def place(self, x: np.ndarray, length: int) -> None:
+        self.x.upload(x)
+        self.lens.upload(np.array([length], np.int32))
+        self.starts.upload(np.array([0, x.shape[0]], np.int32))
+
+    def output(self, rows: int) -> np.ndarray:
+        d.synchronize()
+        return self.y.download(np.float32, (rows, self.hidden))
+
+
+def run(hidden=1024, heads=16, kv_heads=4, dim=64, page=32, prompt=200, steps=4, seed=0):
+    """(layer, prompt's and tokens' inputs and outputs, seconds of the prompt and of a token)."""
+    layer = Layer(hidden, heads, kv_heads, dim, page, prompt + steps, seed)
+    rng = np.random.default_rng(seed + 1)
+    x = rng.standard_normal((prompt + steps, hidden)).astype(np.float32)
+    layer.place(x[:prompt], prompt)
+    t0 = time.perf_counter()
+    layer.enqueue(prompt, prompt, four_bits=True)
+    out = [layer.output(prompt)]
+    t1 = time.perf_counter()
+    for i in range(prompt, prompt + steps):
+        layer.place(x[i:i + 1], i + 1)
+        with d.Graph() as step:
+            layer.enqueue(1, i + 1, four_bits=False)
+        step.launch()
+        out.append(layer.output(1))
+        step.destroy()
+    return layer, x, np.concatenate(out), t1 - t0, (time.perf_counter() - t1) / steps
+
+
+def main() -> int:
+    ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
+    ap.add_argument("--hidden", type=int, default=1024)
+    ap.add_argument("--prompt", type=int, default=200)
+    ap.add_argument("--steps", type=int, default=4)
+    a = ap.parse_args()
+    layer, x, out, first, token = run(hidden=a.hidden, prompt=a.prompt, steps=a.steps)
+    print(f"prompt of {a.prompt}: {first * 1e3:.2f} ms; a token: {token * 1e6:.0f} us; "
+          f"|y| of the last token {np.linalg.norm(out[-1]):.4f}")
+    return 0
+
+
+if __name__ == "__main__":
+    raise SystemExit(main())

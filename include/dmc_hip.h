@@ -309,8 +309,8 @@ int32_t dmc_hip_mxfp4_dequantize(int64_t q_dev, int64_t s_dev, int64_t dst_dev, 
 
 /* y f32 [m,n] = x f32 [m,k] @ W', W [n,k] in MXFP4: dmc_hip_gemv_rd's product on
  * 4-bit weights, any m.  x enters with its 24 bits (of its block of 32's largest
- * value from 6 rows on), products are exact, sums are f32; NaN and inf classes are
- * the formula's.  k == 0 writes +0.0.  From 6 rows on x's digits take a workspace
+ * value from 3 rows on), products are exact, sums are f32; NaN and inf classes are
+ * the formula's.  k == 0 writes +0.0.  From 3 rows on x's digits take a workspace
  * of ceil(m / 16) * ceil(k / 128) * 8192 bytes plus 4 per 32 rows. */
 int32_t dmc_hip_gemv_mxfp4_rd(int64_t x_dev, int64_t wq_dev, int64_t ws_dev, int64_t y_dev, int64_t m,
                               int64_t k, int64_t n);
