@@ -1238,19 +1238,22 @@ hipError_t launch_kv_append(const KvAppend &args, hipStream_t stream) {
 KvPlan plan_kv(const KvAttend &p, int num_cus) {
     KvPlan pl{};
     const int group = p.q_heads / p.c.heads;
-    pl.kind = p.b.max_new * group > 16 ? 1 : 0;
+    // Rows by 16 (f32: by 4) while they are at most two (four) column tiles, each of which reads the codes again: 32
+    // sequences of 2048, 8 tokens x 4 heads, bf16 33 us against 69 in tiles of 128; 4 of 8192, 48 rows 41 against 38;
+    // f32, 24 rows 68 against 40.
+    pl.kind = p.b.max_new * group > (p.bf16 ? 32 : 16) ? 1 : 0;
     const int R = tile_rows(p, pl.kind);
     const int64_t tiles = (int64_t)((p.b.max_new * group + R - 1) / R) * p.c.heads * p.b.batch;
     const int64_t unit = pl.kind ? kStep : 4 * kStep;  // tokens of a workgroup's step
     int64_t span = p.b.max_len;
     if (p.window > 0) span = std::min<int64_t>(span, p.window + R + kStep);
     const int64_t units = std::max<int64_t>(1, (span + unit - 1) / unit);
-    // Few rows: one workgroup per CU, each as long as that allows up to 16 steps of 256 tokens (uneven sequences then
-    // still spread).  One token over 131072: 16 steps 61 us, 8 65, 4 75, 2 97; 64 sequences up to 8192: 144, 153, 153.
-    // Tiles: two per CU, of at least 8 steps, since each writes its partial rows.
+    // Few rows: one workgroup per CU, each as long as that allows up to 32 steps of 256 tokens (uneven sequences then
+    // still spread).  One token over 131072: 16 steps 61 us, 8 65, 4 75, 2 97; 64 sequences up to 8192: 32 steps 122
+    // us, 16 132.  Tiles: two per CU, of at least 8 steps, since each writes its partial rows.
     const int64_t want = std::max<int64_t>(1, (pl.kind ? 2 : 1) * num_cus / std::max<int64_t>(1, tiles));
     int64_t per = (units + want - 1) / want;
-    per = pl.kind ? std::max<int64_t>(per, 8) : std::min<int64_t>(per, 16);
+    per = pl.kind ? std::max<int64_t>(per, 8) : std::min<int64_t>(per, 32);
     per = std::max<int64_t>(per, (units + kMaxSplits - 1) / kMaxSplits);
     pl.chunk = (int)(per * unit);
     pl.splits = (int)((units + per - 1) / per);
