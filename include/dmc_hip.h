@@ -291,7 +291,8 @@ int32_t dmc_hip_bf16_transpose_2d(int64_t src_dev, int64_t dst_dev, int64_t m, i
  * dmc_hip_mxfp4_row_scales(k) bytes apart; what lies past k in a row's last group
  * is code 0 (the quantiser writes it so, and the products rely on it).  Codes are
  * 16-byte aligned, scales 4-byte aligned.  All entries are on device pointers,
- * ordered on the library stream, and may be recorded into a graph. */
+ * ordered on the library stream, and may be recorded into a graph (a call that needs
+ * more workspace than dmc_hip_capture_begin reserves: after one uncaptured call). */
 #define DMC_HIP_F32 0
 #define DMC_HIP_BF16 1
 int64_t dmc_hip_mxfp4_row_bytes(int64_t k);
