@@ -695,9 +695,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_rows_kernel(const Kv
 // read at a time meet different banks.
 //
 // Measured, chunks of up to 2048 tokens of 4 sequences over up to 8192, 32 heads on 8 of
-// 128, bf16: 900 us, 892 TFLOP/s (a large bf16 product: 1207).  MFMAs were busy for
-// 39% of the CUs' cycles at 934 us, before the weights' sums and maxima took their form of
-// now.  At that state 64 rows per workgroup took 1043 us, and wave priorities the same or more.
+// 128, bf16: 900 us, 892 TFLOP/s (a large bf16 product: 1207).  MFMAs are busy for
+// 40% of the CUs' cycles; LDS reads meet no bank twice.  At a state of 929 us, 64 rows per
+// workgroup took 1043, and wave priorities 938.
 template <int D>
 struct KvTile {
     static constexpr int KC = D / 16;                        // pieces of a K row
